@@ -1,0 +1,113 @@
+// Pieces shared by the kernels of linear attention with a decay per head (decay.hip): launch
+// descriptors, operand fragments for bf16 and fp32, LDS tiles and their staging.
+//
+// Fragments.  A 16x16 product over 32 contraction indices takes eight of them per lane: lane l holds
+// row (A) or column (B) l % 16 and the indices of group g = l / 16.  bf16: one v_mfma_f32_16x16x32_bf16.
+// fp32: eight v_mfma_f32_16x16x4_f32, the e-th over element e of the four groups; any assignment of
+// indices to (g, e) will do as long as A and B agree, so both types share one layout.
+#pragma once
+
+#include "la_common.hpp"
+#include "la_internal.hpp"
+
+namespace la {
+
+constexpr int kDecayC = 64;        // tokens per chunk
+
+struct f32x8 {
+  float v[8];
+};
+
+__device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <bool F32>
+struct DecayOps;
+
+template <>
+struct DecayOps<false> {
+  typedef uint16_t elem;
+  typedef u32x4 frag;
+  static constexpr int kPad = 8;         // elements behind a row of an LDS tile
+  static constexpr int kPair = 2;        // parts of a score or state entry in a bf16 product
+  static constexpr int kFine = 3;        // parts of a weighted value in the state's update
+  static __device__ __forceinline__ f32x4 mma(const frag& a, const frag& b, f32x4 c) { return mfma16x16x32(a, b, c); }
+  static __device__ __forceinline__ frag row(const elem* p) { return *reinterpret_cast<const u32x4*>(p); }
+  static __device__ __forceinline__ frag rows4(const elem* p0, const elem* p1) {
+    const u32x2 a = *reinterpret_cast<const u32x2*>(p0), b = *reinterpret_cast<const u32x2*>(p1);
+    return (u32x4){a[0], a[1], b[0], b[1]};
+  }
+  // Column c0 + l % 16 of rows row0 + 8 g .. + 7 of a row-major tile: two transposed reads of four rows,
+  // in each of which a 16-lane group's lane i addresses four columns of row i / 4.
+  static __device__ __forceinline__ frag col(const elem* tile, int ld, int row0, int c0, int lane) {
+    typedef short v4s __attribute__((ext_vector_type(4)));
+    const int i = lane & 15, g = lane >> 4;
+    const elem* p = tile + (row0 + 8 * g + (i >> 2)) * ld + c0 + 4 * (i & 3);
+    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)p));
+    const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(p + 4 * ld)));
+    return (u32x4){a[0], a[1], b[0], b[1]};
+  }
+  static __device__ __forceinline__ f32x8 widen(const frag& a) {
+    f32x8 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      r.v[2 * i] = bf16_lo_to_f32(a[i]);
+      r.v[2 * i + 1] = bf16_hi_to_f32(a[i]);
+    }
+    return r;
+  }
+  // x as P bf16 terms, x = p[0] + p[1] + .. : 8, 16 or 24 significant bits
+  template <int P>
+  static __device__ __forceinline__ void parts(f32x8 x, frag (&p)[P]) {
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[j][i] = pack_bf16x2(x.v[2 * i], x.v[2 * i + 1]);
+        if (j + 1 < P) {
+          x.v[2 * i] -= bf16_lo_to_f32(p[j][i]);
+          x.v[2 * i + 1] -= bf16_hi_to_f32(p[j][i]);
+        }
+      }
+  }
+};
+
+template <>
+struct DecayOps<true> {
+  typedef float elem;
+  typedef f32x8 frag;
+  static constexpr int kPad = 4;
+  static constexpr int kPair = 1;
+  static constexpr int kFine = 1;
+  static __device__ __forceinline__ f32x4 mma(const frag& a, const frag& b, f32x4 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e], b.v[e], c, 0, 0, 0);
+    return c;
+  }
+  static __device__ __forceinline__ frag row(const elem* p) { return rows4(p, p + 4); }
+  static __device__ __forceinline__ frag rows4(const elem* p0, const elem* p1) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p0), b = *reinterpret_cast<const f32x4*>(p1);
+    return {{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
+  }
+  static __device__ __forceinline__ frag col(const elem* tile, int ld, int row0, int c0, int lane) {
+    const elem* p = tile + (row0 + 8 * (lane >> 4)) * ld + c0 + (lane & 15);
+    frag r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r.v[e] = p[e * ld];
+    return r;
+  }
+  static __device__ __forceinline__ f32x8 widen(const frag& a) { return a; }
+  template <int P>
+  static __device__ __forceinline__ void parts(const f32x8& x, frag (&p)[P]) {
+    static_assert(P == 1, "fp32 operands are exact");
+    p[0] = x;
+  }
+};
+
+// A (B, H, N, w) operand: element (b, h, t, i) at p + b s[0] + h s[1] + t s[2] + i.
+struct DecayTensor {
+  const void* p;
+  long long s[3];
+  int vec;      // rows of 16-byte pieces: start, strides and width allow 16-byte loads
+};
+
+}  // namespace la

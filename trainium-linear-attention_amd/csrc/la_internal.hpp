@@ -89,6 +89,40 @@ struct DecodeArgs {
   bool normalize, in_f32, out_f32;
 };
 
+struct DecayArgs {       // la_decay_fwd, la_decay_bwd
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;                // forward
+  const void* dout;         // backward
+  void* dq;
+  void* dk;
+  void* dv_out;
+  const float* state_in;    // optional, (B, H, d, dv) fp32, as the next three
+  float* state_out;
+  const float* dstate_out;
+  float* dstate_in;
+  const float* log_decay;   // (H)
+  const int* lengths;       // optional, (B)
+  long long q_strides[3], k_strides[3], v_strides[3], dout_strides[3];   // elements: batch, head, token
+  void* workspace;          // decay_workspace_bytes()
+  int B, H, N, d, dv;
+  float scale;
+  bool in_f32, out_f32;
+};
+
+struct DecayStepArgs {
+  const void* q;            // (BH, d)
+  const void* k;
+  const void* v;            // (BH, dv)
+  const float* log_decay;   // (H)
+  float* state;             // (BH, d, dv) fp32, updated in place
+  void* out;
+  int B, H, d, dv;
+  float scale;
+  bool in_f32, out_f32;
+};
+
 struct FeatureMapArgs {
   const void* x;
   void* out;
@@ -153,6 +187,10 @@ int device_cu_count();   // compute units of the current device (256 when the qu
 bool identity_shape(int d, int dv);
 size_t identity_workspace_bytes(int BH, int N, int d, int dv);
 int launch_identity(const IdentityArgs& a, hipStream_t stream);
+size_t decay_workspace_bytes(long long BH, int N, int d, int dv);
+int launch_decay_fwd(const DecayArgs& a, hipStream_t stream);
+int launch_decay_bwd(const DecayArgs& a, hipStream_t stream);
+int launch_decay_step(const DecayStepArgs& a, hipStream_t stream);
 bool decode_shape(int d, int dv);
 int launch_decode_step(const DecodeArgs& a, hipStream_t stream);
 size_t decode_workspace_bytes(long long BH, int d, int dv);

@@ -5,6 +5,7 @@ from .based_layer import based_layer_attn
 from .based_module import TrainiumBasedLinearAttention, TrainiumBasedLinearAttentionNKI
 from .chunked_attention import (based_chunked, based_decode_step, chunked_based_attn, chunked_nki_numerator,
                                 feature_dim, taylor_feature_map)
+from .decay_attention import decay_decode_step, decay_linear_attn
 from .identity_attention import identity_linear_attn
 from .pytorch_attention import based_parallel, solution, solution_nki
 from .sliding_attention import nki_sliding_window_attn, sliding_window_attn
@@ -15,4 +16,5 @@ __all__ = [
     "nki_sliding_window_attn", "sliding_window_attn",
     "TrainiumBasedLinearAttention", "TrainiumBasedLinearAttentionNKI", "based_layer_attn",
     "identity_linear_attn", "based_decode_step",
+    "decay_linear_attn", "decay_decode_step",
 ]

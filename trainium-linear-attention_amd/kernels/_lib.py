@@ -1,4 +1,5 @@
-"""ctypes binding of libbased_la.so (the C ABI declared in include/based_la.h and based_la_ext.h).
+"""ctypes binding of libbased_la.so (the C ABI declared in include/based_la.h, based_la_ext.h,
+based_la_decay.h and based_la_cache.h).
 
 The library is loaded lazily, after ``import torch`` so that its HIP runtime dependency
 resolves to the runtime torch has already mapped; launches go on torch's current stream.
@@ -78,6 +79,15 @@ _SIGNATURES = {
                                                _c_size, _c_void]),
     "la_based_parallel_strided_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_void, _c_void,
                                                             _c_void]),
+    "la_decay_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int]),
+    "la_decay_fwd": (_c_int, [_c_void, _c_void, _c_void, _c_int, _c_void, _c_int, _c_int, _c_int, _c_int, _c_int,
+                              _c_int, _c_void, _c_void, _c_void, _c_void, _c_void, _c_float, _c_void, _c_void,
+                              _c_void, _c_size, _c_void]),
+    "la_decay_bwd": (_c_int, [_c_void, _c_void, _c_void, _c_void, _c_int, _c_void, _c_void, _c_void, _c_int, _c_int,
+                              _c_int, _c_int, _c_int, _c_void, _c_void, _c_void, _c_void, _c_void, _c_void, _c_float,
+                              _c_void, _c_void, _c_void, _c_void, _c_size, _c_void]),
+    "la_decay_step": (_c_int, [_c_void, _c_void, _c_void, _c_int, _c_void, _c_void, _c_void, _c_int, _c_int, _c_int,
+                               _c_int, _c_int, _c_float, _c_void]),
     "la_taylor_feature_map": (_c_int, [_c_void, _c_int, _c_void, _c_int, ctypes.c_longlong, _c_int, _c_void]),
 }
 
