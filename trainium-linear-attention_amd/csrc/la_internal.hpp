@@ -123,6 +123,25 @@ struct DecayStepArgs {
   bool in_f32, out_f32;
 };
 
+struct SlidingCacheArgs {   // la_sliding_cache_append, la_sliding_decode_step
+  const void* q;            // (B, H, d), the step's, as the next
+  void* out;
+  const void* k;
+  const void* v;
+  void* kc;
+  void* vc;
+  float* ks;
+  float* vs;
+  const int* start;         // the append's, optional, (B)
+  const int* lengths;       // append: optional, new tokens; step: whole sequences (last_of)
+  bool last_of;
+  long long k_strides[3], v_strides[3];
+  void* workspace;          // sliding_decode_workspace_bytes()
+  int B, H, HK, N, d, dv, blocks, window;
+  float scale;
+  bool in_f32, out_f32;
+};
+
 struct FeatureMapArgs {
   const void* x;
   void* out;
@@ -191,6 +210,10 @@ size_t decay_workspace_bytes(long long BH, int N, int d, int dv);
 int launch_decay_fwd(const DecayArgs& a, hipStream_t stream);
 int launch_decay_bwd(const DecayArgs& a, hipStream_t stream);
 int launch_decay_step(const DecayStepArgs& a, hipStream_t stream);
+int sliding_cache_dim(int d);   // a cache row's codes: 32, 64 or 128
+size_t sliding_decode_workspace_bytes(int B, int H, int HK, int dv, int blocks, int window);
+int launch_sliding_append(const SlidingCacheArgs& a, hipStream_t stream);
+int launch_sliding_decode(const SlidingCacheArgs& a, hipStream_t stream);
 bool decode_shape(int d, int dv);
 int launch_decode_step(const DecodeArgs& a, hipStream_t stream);
 size_t decode_workspace_bytes(long long BH, int d, int dv);

@@ -1,0 +1,508 @@
+// An 8-bit cache of keys and values and one-token softmax attention over it, for gfx950.  The layout is
+// based_la_cache.h's: blocks of 64 tokens, e4m3 codes with a power-of-two scale for each block and head, the
+// values of a block transposed.
+//
+// Why this layout: a wave takes a block at a time, and every operand of its products is a 16-byte load of
+// consecutive codes.  S^T = K Q^T has the block's keys as rows and up to 16 query heads as columns; of its four
+// tiles of 16 keys, row 4 g + r of tile m is key 16 g + 4 m + r, so that lane group g ends up with the scores of
+// keys 16 g .. + 15, which is the order in which it holds V^T's codes (16 consecutive keys of a value column)
+// for O^T = V^T P^T.  Nothing is transposed or passed through LDS before the waves' results are joined.
+// Power-of-two scales make x / scale exact, so that a code is rounded once, and codes that move to a larger
+// scale only round where they fall below e4m3's normal range.
+#include <math.h>
+
+#include <algorithm>
+
+#include "la_common.hpp"
+#include "la_decay.hpp"
+#include "la_internal.hpp"
+
+namespace la {
+
+namespace {
+
+constexpr int CB = 64;       // tokens of a block
+
+// Exponent of the smallest power of two, 2^-100 at the least, that brings a magnitude (as bits) to 448 = 1.75 2^8
+// or below.
+__device__ __forceinline__ int scale_exp(u32 bits) {
+  return max((int)(bits >> 23) - 135 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0), -100);
+}
+__device__ __forceinline__ float pow2f(int e) { return __builtin_bit_cast(float, (u32)(e + 127) << 23); }
+// 1 / s for a power of two within 2^-126 .. 2^126
+__device__ __forceinline__ float inv_pow2(float s) { return __builtin_bit_cast(float, 0x7f000000u - __builtin_bit_cast(u32, s)); }
+__device__ __forceinline__ u32 finite_mag(float x) {
+  const u32 m = __builtin_bit_cast(u32, x) & 0x7fffffffu;
+  return m < 0x7f800000u ? m : 0u;
+}
+
+// Four values to four codes; what no code stands for (infinities) becomes NaN.
+__device__ __forceinline__ u32 encode4(float a, float b, float c, float d) {
+  const float nan = __builtin_nanf("");
+  a = fabsf(a) > 448.f ? nan : a;
+  b = fabsf(b) > 448.f ? nan : b;
+  c = fabsf(c) > 448.f ? nan : c;
+  d = fabsf(d) > 448.f ? nan : d;
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (u32)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+}
+__device__ __forceinline__ u32 rescale4(u32 w, float f) {
+  return encode4(__builtin_amdgcn_cvt_f32_fp8((int)w, 0) * f, __builtin_amdgcn_cvt_f32_fp8((int)w, 1) * f,
+                 __builtin_amdgcn_cvt_f32_fp8((int)w, 2) * f, __builtin_amdgcn_cvt_f32_fp8((int)w, 3) * f);
+}
+
+struct CacheParams {
+  DecayTensor k, v;
+  uint8_t* kc;
+  uint8_t* vc;
+  float* ks;
+  float* vs;
+  const int* start;
+  const int* lengths;
+  int last_of;       // lengths are whole sequences', of which the last token is appended
+  int HK, N, d, dv, blocks, in_f32;
+};
+
+struct f8 {
+  float v[8];
+};
+
+// Elements col .. col + 7 of a row of w, zeros behind it.
+__device__ __forceinline__ f8 load8(const DecayTensor& x, size_t at, int col, int w, bool there, int f32) {
+  f8 r;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r.v[j] = 0.f;
+  if (!there || col >= w) return r;
+  if (f32) {
+    const float* s = static_cast<const float*>(x.p) + at + col;
+    if (x.vec && col + 8 <= w) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(s), b = *reinterpret_cast<const f32x4*>(s + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r.v[j] = a[j], r.v[4 + j] = b[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (col + j < w) r.v[j] = s[j];
+    }
+  } else {
+    const uint16_t* s = static_cast<const uint16_t*>(x.p) + at + col;
+    if (x.vec) {
+      const u32x4 a = *reinterpret_cast<const u32x4*>(s);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r.v[2 * j] = bf16_lo_to_f32(a[j]), r.v[2 * j + 1] = bf16_hi_to_f32(a[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (col + j < w) r.v[j] = bf16_bits_to_f32(s[j]);
+    }
+  }
+  return r;
+}
+
+// One block of one (sequence, cached head): blockIdx.x the block among those the call touches.
+template <int DP, int DVP>
+__global__ __launch_bounds__(256) void cache_append_kernel(const CacheParams p) {
+  constexpr int KI = CB * DP / 8 / 256, VI = CB * DVP / 8 / 256, VROW = CB + 4;
+  __shared__ u32 top[2][4];
+  __shared__ __attribute__((aligned(16))) uint8_t vt[DVP * VROW];
+  const int tid = threadIdx.x, bh = blockIdx.y, b = bh / p.HK, hk = bh - b * p.HK;
+  int from = p.start ? p.start[b] : 0, n = p.lengths ? min(max(p.lengths[b], 0), p.N) : p.N;
+  if (p.last_of) {
+    from = p.lengths[b] - 1;
+    n = from >= 0 ? 1 : 0;
+  }
+  const int lb = from / CB + blockIdx.x, end = from + n;      // tokens from .. end - 1
+  if (n <= 0 || from < 0 || lb * CB >= end) return;
+  if (lb + p.blocks <= (end - 1) / CB) return;                // taken over later in this call
+  const int kept = max(from - lb * CB, 0), stop = min(end - lb * CB, CB);
+  const size_t rec = (size_t)bh * p.blocks + lb % p.blocks;
+  const size_t kb = (size_t)(b * p.k.s[0] + hk * p.k.s[1]), vb = (size_t)(b * p.v.s[0] + hk * p.v.s[1]);
+  uint8_t* kc = p.kc + rec * (CB * DP);
+  uint8_t* vc = p.vc + rec * (CB * DVP);
+
+  f8 kx[KI], vx[VI];
+  u32 km = 0, vm = 0;
+#pragma unroll
+  for (int i = 0; i < KI; ++i) {
+    const int at = tid + 256 * i, row = at / (DP / 8), t = lb * CB + row - from;
+    kx[i] = load8(p.k, kb + (size_t)t * p.k.s[2], at % (DP / 8) * 8, p.d, row >= kept && row < stop, p.in_f32);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) km = max(km, finite_mag(kx[i].v[j]));
+  }
+#pragma unroll
+  for (int i = 0; i < VI; ++i) {
+    const int at = tid + 256 * i, row = at / (DVP / 8), t = lb * CB + row - from;
+    vx[i] = load8(p.v, vb + (size_t)t * p.v.s[2], at % (DVP / 8) * 8, p.dv, row >= kept && row < stop, p.in_f32);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) vm = max(vm, finite_mag(vx[i].v[j]));
+  }
+  km = wave_max_u32(km);
+  vm = wave_max_u32(vm);
+  if ((tid & 63) == 0) {
+    top[0][tid >> 6] = km;
+    top[1][tid >> 6] = vm;
+  }
+  const float old_k = kept ? p.ks[rec] : 0.f, old_v = kept ? p.vs[rec] : 0.f;
+  __syncthreads();
+  km = max(max(top[0][0], top[0][1]), max(top[0][2], top[0][3]));
+  vm = max(max(top[1][0], top[1][1]), max(top[1][2], top[1][3]));
+  const float sk = fmaxf(pow2f(scale_exp(km)), old_k), sv = fmaxf(pow2f(scale_exp(vm)), old_v);
+  const float ik = inv_pow2(sk), iv = inv_pow2(sv);
+  if (tid == 0) {
+    p.ks[rec] = sk;
+    p.vs[rec] = sv;
+  }
+#pragma unroll
+  for (int i = 0; i < KI; ++i) {
+    const int at = tid + 256 * i, row = at / (DP / 8);
+    u32x2* dst = reinterpret_cast<u32x2*>(kc + 8 * at);
+    u32x2 w;
+    if (row < kept) {
+      w = *dst;
+      w = (u32x2){rescale4(w[0], old_k * ik), rescale4(w[1], old_k * ik)};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) kx[i].v[j] *= ik;
+      w = (u32x2){encode4(kx[i].v[0], kx[i].v[1], kx[i].v[2], kx[i].v[3]), encode4(kx[i].v[4], kx[i].v[5], kx[i].v[6], kx[i].v[7])};
+    }
+    *dst = w;
+  }
+#pragma unroll
+  for (int i = 0; i < VI; ++i) {
+    const int at = tid + 256 * i, row = at / (DVP / 8), col = at % (DVP / 8) * 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) vx[i].v[j] *= iv;
+    const u32 w0 = encode4(vx[i].v[0], vx[i].v[1], vx[i].v[2], vx[i].v[3]), w1 = encode4(vx[i].v[4], vx[i].v[5], vx[i].v[6], vx[i].v[7]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      vt[(col + j) * VROW + row] = (uint8_t)(w0 >> (8 * j));
+      vt[(col + 4 + j) * VROW + row] = (uint8_t)(w1 >> (8 * j));
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < DVP * CB / 4; i += 256) {
+    const int col = i / (CB / 4), t = i % (CB / 4) * 4;
+    u32* dst = reinterpret_cast<u32*>(vc + col * CB + t);
+    u32 w = *reinterpret_cast<const u32*>(vt + col * VROW + t);
+    if (t < kept) {
+      const u32 o = rescale4(*dst, old_v * iv), m = kept - t >= 4 ? 0xffffffffu : (1u << (8 * (kept - t))) - 1;
+      w = (w & ~m) | (o & m);
+    }
+    *dst = w;
+  }
+}
+
+// ---- attention
+
+struct StepParams {
+  const void* q;
+  void* out;
+  const uint8_t* kc;
+  const uint8_t* vc;
+  const float* ks;
+  const float* vs;
+  const int* lengths;
+  float* part;       // (B H, splits, DVP + 2): O, maximum, sum; or null: one split
+  int H, HK, G, d, dv, blocks, window, splits;
+  float scale;
+  int in_f32, out_f32;
+};
+
+typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf2;
+
+// Eight codes as eight bf16 values (exact)
+__device__ __forceinline__ u32x4 codes_bf16(u32 a, u32 b) {
+  return (u32x4){__builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false)),
+                 __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true)),
+                 __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false)),
+                 __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true))};
+}
+
+// Bytes t .. t + 3 of a mask of valid places lo .. hi - 1.
+__device__ __forceinline__ u32 byte_mask(int t, int lo, int hi) {
+  u32 m = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) m |= t + j >= lo && t + j < hi ? 0xffu << (8 * j) : 0u;
+  return m;
+}
+
+// Work-group: up to 16 query heads of one cached head of one sequence, one split of its blocks, which the four
+// waves take in turn.  F32: q as three bf16 terms and P as three; bf16 q is itself, P two (16 bits).
+template <bool F32, int DP, int DVP>
+__global__ __launch_bounds__(256) void cache_attn_kernel(const StepParams p) {
+  constexpr int NQ = F32 ? 3 : 1, NP = F32 ? 3 : 2, KS = DP / 32, MT = DVP / 16;
+  constexpr int KL = DP >= 64 ? DP / 64 : 1;       // loads of a key row per lane, of 16 (DP = 32: 8) bytes
+  __shared__ float ms[4][16], ls[4][16];
+  __shared__ float os[4][DVP][17];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, g = lane >> 4;
+  const int split = blockIdx.x, ng = (p.G + 15) / 16, hk = blockIdx.y / ng, hg = blockIdx.y - hk * ng, b = blockIdx.z;
+  const int h0 = hk * p.G + 16 * hg, nh = min(16, p.G - 16 * hg);      // query heads h0 .. h0 + nh - 1
+  const int len = p.lengths[b], last = len - 1;
+  // positions p0 .. last, in blocks b0 .. b1 - 1; this split's of them
+  int p0 = max(0, (last / CB + 1 - p.blocks) * CB);
+  if (p.window > 0) p0 = max(p0, len - p.window);
+  const int b0 = p0 / CB, nb = len > 0 ? last / CB + 1 - b0 : 0, per = (nb + p.splits - 1) / p.splits;
+  const int s0 = b0 + split * per, s1 = min(b0 + nb, s0 + per);
+
+  // Q^T: head n16, dims in the order of the key loads
+  u32x4 qf[KS][NQ];
+#pragma unroll
+  for (int x = 0; x < KS; ++x) {
+    const int c = DP >= 64 ? 64 * (x / 2) + 16 * g + 8 * (x & 1) : 8 * g;
+    f32x8 y;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      y.v[j] = 0.f;
+      if (n16 < nh && c + j < p.d) {
+        const size_t at = ((size_t)b * p.H + h0 + n16) * p.d + c + j;
+        y.v[j] = p.in_f32 ? static_cast<const float*>(p.q)[at] : bf16_bits_to_f32(static_cast<const uint16_t*>(p.q)[at]);
+      }
+    }
+    DecayOps<false>::parts<NQ>(y, qf[x]);
+  }
+
+  float m = -INFINITY, l = 0.f;
+  f32x4 o[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) o[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  const float c2 = p.scale * 1.44269504088896341f;
+  for (int blk = s0 + w; blk < s1; blk += 4) {
+    const size_t rec = ((size_t)b * p.HK + hk) * p.blocks + blk % p.blocks;
+    const uint8_t* kc = p.kc + rec * (CB * DP);
+    const uint8_t* vc = p.vc + rec * (CB * DVP);
+    u32x4 kx[4][KL], vx[MT];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const uint8_t* row = kc + ((n16 >> 2) * 16 + 4 * t + (n16 & 3)) * DP;
+#pragma unroll
+      for (int c = 0; c < KL; ++c) {
+        if constexpr (DP >= 64) {
+          kx[t][c] = *reinterpret_cast<const u32x4*>(row + 64 * c + 16 * g);
+        } else {
+          const u32x2 y = *reinterpret_cast<const u32x2*>(row + 8 * g);
+          kx[t][c] = (u32x4){y[0], y[1], 0u, 0u};
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) vx[t] = *reinterpret_cast<const u32x4*>(vc + (16 * t + n16) * CB + 16 * g);
+    const float ksc = p.ks[rec] * c2, vsc = p.vs[rec];
+    f32x4 s[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      s[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < KS; ++x) {
+        const u32x4 kf = codes_bf16(kx[t][x / 2][2 * (x & 1)], kx[t][x / 2][2 * (x & 1) + 1]);
+#pragma unroll
+        for (int j = NQ - 1; j >= 0; --j) s[t] = mfma16x16x32(kf, qf[x][j], s[t]);
+      }
+    }
+    const int lo = p0 - blk * CB, hi = len - blk * CB;     // valid places of the block
+    const bool edge = lo > 0 || hi < CB;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[t][r] *= ksc;
+        if (edge) {
+          const int key = 16 * g + 4 * t + r;
+          if (key < lo || key >= hi) s[t][r] = -INFINITY;
+        }
+        mx = fmaxf(mx, s[t][r]);
+      }
+    mx = fmaxf(mx, __shfl_xor(mx, 16));
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn, fade = exp2_raw(m - ref);
+    m = mn;
+    l *= fade;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) o[t] *= fade;
+    u32x4 pf[2][NP];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      f32x8 y;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float e = exp2_raw(s[2 * x + j / 4][j % 4] - ref);
+        l += e;
+        y.v[j] = e * vsc;
+      }
+      DecayOps<false>::parts<NP>(y, pf[x]);
+    }
+    if (edge) {      // places that hold no token of the window may hold anything
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const u32 mask = byte_mask(16 * g + 4 * j, lo, hi);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) vx[t][j] &= mask;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const u32x4 vf = codes_bf16(vx[t][2 * x], vx[t][2 * x + 1]);
+#pragma unroll
+        for (int j = NP - 1; j >= 0; --j) o[t] = mfma16x16x32(vf, pf[x][j], o[t]);
+      }
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  // join the waves
+  if (g == 0) {
+    ms[w][n16] = m;
+    ls[w][n16] = l;
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) os[w][16 * t + 4 * g + r][n16] = o[t][r];
+  __syncthreads();
+  for (int i = tid; i < nh * DVP; i += 256) {
+    const int h = i / DVP, c = i % DVP;
+    const float mm = fmaxf(fmaxf(ms[0][h], ms[1][h]), fmaxf(ms[2][h], ms[3][h])), ref = mm == -INFINITY ? 0.f : mm;
+    float sum = 0.f, y = 0.f;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float f = exp2_raw(ms[x][h] - ref);
+      sum = __builtin_fmaf(ls[x][h], f, sum);
+      y = __builtin_fmaf(os[x][c][h], f, y);
+    }
+    const size_t head = (size_t)b * p.H + h0 + h;
+    if (p.part != nullptr) {
+      float* dst = p.part + (head * p.splits + split) * (DVP + 2);
+      dst[c] = y;
+      if (c == 0) {
+        dst[DVP] = mm;
+        dst[DVP + 1] = sum;
+      }
+    } else if (c < p.dv) {
+      y = nb > 0 ? y / sum : 0.f;
+      if (p.out_f32) static_cast<float*>(p.out)[head * p.dv + c] = y;
+      else static_cast<uint16_t*>(p.out)[head * p.dv + c] = f32_to_bf16_bits(y);
+    }
+  }
+}
+
+// A head's splits, in order.
+template <int DVP>
+__global__ __launch_bounds__(DVP < 64 ? 64 : DVP) void cache_combine_kernel(const StepParams p) {
+  const size_t head = blockIdx.x;
+  const int c = threadIdx.x;
+  const float* src = p.part + head * p.splits * (DVP + 2);
+  float m = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, src[s * (DVP + 2) + DVP]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float sum = 0.f, y = 0.f;
+  for (int s = 0; s < p.splits; ++s) {
+    const float f = exp2_raw(src[s * (DVP + 2) + DVP] - ref);
+    sum = __builtin_fmaf(src[s * (DVP + 2) + DVP + 1], f, sum);
+    if (c < DVP) y = __builtin_fmaf(src[s * (DVP + 2) + c], f, y);
+  }
+  if (c >= p.dv) return;
+  y = p.lengths[head / p.H] > 0 ? y / sum : 0.f;
+  if (p.out_f32) static_cast<float*>(p.out)[head * p.dv + c] = y;
+  else static_cast<uint16_t*>(p.out)[head * p.dv + c] = f32_to_bf16_bits(y);
+}
+
+template <int DP, int DVP>
+int launch_append(const CacheParams& p, int BHK, hipStream_t stream) {
+  const int nb = (p.N + 2 * CB - 2) / CB;       // blocks that N tokens may touch
+  hipLaunchKernelGGL((cache_append_kernel<DP, DVP>), dim3((unsigned)nb, (unsigned)BHK), dim3(256), 0, stream, p);
+  return (int)hipGetLastError();
+}
+
+template <bool F32, int DP, int DVP>
+int launch_attn(const StepParams& p, int B, hipStream_t stream) {
+  const dim3 grid((unsigned)p.splits, (unsigned)(p.HK * ((p.G + 15) / 16)), (unsigned)B);
+  hipLaunchKernelGGL((cache_attn_kernel<F32, DP, DVP>), grid, dim3(256), 0, stream, p);
+  if (p.part != nullptr)
+    hipLaunchKernelGGL((cache_combine_kernel<DVP>), dim3((unsigned)(B * p.H)), dim3(DVP < 64 ? 64 : DVP), 0, stream, p);
+  return (int)hipGetLastError();
+}
+
+#define LA_CACHE_DIMS(CALL)                                   \
+  if (dp == 32 && dvp == 32) return CALL(32, 32);             \
+  if (dp == 32 && dvp == 64) return CALL(32, 64);             \
+  if (dp == 32 && dvp == 128) return CALL(32, 128);           \
+  if (dp == 64 && dvp == 32) return CALL(64, 32);             \
+  if (dp == 64 && dvp == 64) return CALL(64, 64);             \
+  if (dp == 64 && dvp == 128) return CALL(64, 128);           \
+  if (dp == 128 && dvp == 32) return CALL(128, 32);           \
+  if (dp == 128 && dvp == 64) return CALL(128, 64);           \
+  return CALL(128, 128);
+
+int append_dims(const CacheParams& p, int BHK, hipStream_t stream) {
+  const int dp = sliding_cache_dim(p.d), dvp = sliding_cache_dim(p.dv);
+#define LA_CALL(A, B) launch_append<A, B>(p, BHK, stream)
+  LA_CACHE_DIMS(LA_CALL)
+#undef LA_CALL
+}
+
+template <bool F32>
+int attn_dims(const StepParams& p, int B, hipStream_t stream) {
+  const int dp = sliding_cache_dim(p.d), dvp = sliding_cache_dim(p.dv);
+#define LA_CALL(A, C) launch_attn<F32, A, C>(p, B, stream)
+  LA_CACHE_DIMS(LA_CALL)
+#undef LA_CALL
+}
+
+// Splits of a sequence's blocks: work-groups for about two a CU, four blocks each at least.
+int decode_splits(int B, int H, int HK, int blocks, int window) {
+  const long long groups = (long long)B * HK * ((H / HK + 15) / 16);
+  const long long most = window > 0 ? std::min<long long>(blocks, (window + 2 * CB - 2) / CB) : blocks;
+  const long long want = (2LL * device_cu_count() + groups - 1) / groups;
+  return (int)std::max(1LL, std::min(want, (most + 3) / 4));
+}
+
+}  // namespace
+
+int sliding_cache_dim(int d) { return d < 1 || d > 128 ? 0 : d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+
+size_t sliding_decode_workspace_bytes(int B, int H, int HK, int dv, int blocks, int window) {
+  const int s = decode_splits(B, H, HK, blocks, window);
+  return s > 1 ? (size_t)B * H * s * (sliding_cache_dim(dv) + 2) * sizeof(float) : 0;
+}
+
+int launch_sliding_append(const SlidingCacheArgs& a, hipStream_t stream) {
+  const int e = a.in_f32 ? 4 : 8;
+  auto operand = [&](const void* ptr, const long long* s, int w) {
+    DecayTensor x{ptr, {s[0], s[1], s[2]}, 0};
+    x.vec = (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && w % e == 0 && s[0] % e == 0 && s[1] % e == 0 && s[2] % e == 0;
+    return x;
+  };
+  const CacheParams p{operand(a.k, a.k_strides, a.d), operand(a.v, a.v_strides, a.dv), static_cast<uint8_t*>(a.kc),
+                      static_cast<uint8_t*>(a.vc), a.ks, a.vs, a.start, a.lengths, a.last_of ? 1 : 0, a.HK, a.N, a.d, a.dv,
+                      a.blocks, a.in_f32 ? 1 : 0};
+  return append_dims(p, a.B * a.HK, stream);
+}
+
+int launch_sliding_decode(const SlidingCacheArgs& a, hipStream_t stream) {
+  const int rc = launch_sliding_append(a, stream);
+  if (rc != 0) return rc;
+  StepParams p{};
+  p.q = a.q;
+  p.out = a.out;
+  p.kc = static_cast<const uint8_t*>(a.kc);
+  p.vc = static_cast<const uint8_t*>(a.vc);
+  p.ks = a.ks;
+  p.vs = a.vs;
+  p.lengths = a.lengths;
+  p.H = a.H;
+  p.HK = a.HK;
+  p.G = a.H / a.HK;
+  p.d = a.d;
+  p.dv = a.dv;
+  p.blocks = a.blocks;
+  p.window = a.window;
+  p.splits = decode_splits(a.B, a.H, a.HK, a.blocks, a.window);
+  p.part = p.splits > 1 ? static_cast<float*>(a.workspace) : nullptr;
+  p.scale = a.scale;
+  p.in_f32 = a.in_f32 ? 1 : 0;
+  p.out_f32 = a.out_f32 ? 1 : 0;
+  return a.in_f32 ? attn_dims<true>(p, a.B, stream) : attn_dims<false>(p, a.B, stream);
+}
+
+}  // namespace la

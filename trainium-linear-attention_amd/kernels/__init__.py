@@ -9,6 +9,7 @@ from .decay_attention import decay_decode_step, decay_linear_attn
 from .identity_attention import identity_linear_attn
 from .pytorch_attention import based_parallel, solution, solution_nki
 from .sliding_attention import nki_sliding_window_attn, sliding_window_attn
+from .sliding_cache import SlidingCache, sliding_cache, sliding_cache_append, sliding_decode_step
 
 __all__ = [
     "solution_nki", "solution", "based_parallel",
@@ -17,4 +18,5 @@ __all__ = [
     "TrainiumBasedLinearAttention", "TrainiumBasedLinearAttentionNKI", "based_layer_attn",
     "identity_linear_attn", "based_decode_step",
     "decay_linear_attn", "decay_decode_step",
+    "SlidingCache", "sliding_cache", "sliding_cache_append", "sliding_decode_step",
 ]

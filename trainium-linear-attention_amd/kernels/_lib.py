@@ -88,6 +88,13 @@ _SIGNATURES = {
                               _c_void, _c_void, _c_void, _c_void, _c_size, _c_void]),
     "la_decay_step": (_c_int, [_c_void, _c_void, _c_void, _c_int, _c_void, _c_void, _c_void, _c_int, _c_int, _c_int,
                                _c_int, _c_int, _c_float, _c_void]),
+    "la_sliding_cache_dim": (_c_int, [_c_int]),
+    "la_sliding_cache_append": (_c_int, [_c_void, _c_void, _c_int, _c_void, _c_void, _c_void, _c_void, _c_void, _c_void,
+                                         _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void, _c_void, _c_void]),
+    "la_sliding_decode_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
+    "la_sliding_decode_step": (_c_int, [_c_void, _c_void, _c_void, _c_int, _c_void, _c_int, _c_void, _c_void, _c_void,
+                                        _c_void, _c_void, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                        _c_float, _c_void, _c_size, _c_void]),
     "la_taylor_feature_map": (_c_int, [_c_void, _c_int, _c_void, _c_int, ctypes.c_longlong, _c_int, _c_void]),
 }
 
