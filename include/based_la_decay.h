@@ -22,9 +22,9 @@
 extern "C" {
 #endif
 
-/* Scratch of la_decay_fwd and of la_decay_bwd (either call), 16-byte aligned; 0 for short sequences, for
+/* Scratch of la_decay_fwd, or of la_decay_bwd (backward = 1), 16-byte aligned; 0 for short sequences, for
  * batches of many heads and for sizes outside the limits: NULL is then accepted. */
-size_t la_decay_workspace_bytes(int B, int H, int N, int d, int dv);
+size_t la_decay_workspace_bytes(int B, int H, int N, int d, int dv, int backward);
 
 /*
  * y and, if state_out is given, the state after the last token.  state_in NULL: zero.  state_out must

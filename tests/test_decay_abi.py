@@ -30,10 +30,10 @@ def test_exports():
 
 def test_workspace_sizes():
     lib = _lib()
-    assert lib.la_decay_workspace_bytes(1, 1, 64, 64, 64) == 0
-    assert lib.la_decay_workspace_bytes(1, 4, 8192, 64, 64) > 0
+    assert lib.la_decay_workspace_bytes(1, 1, 64, 64, 64, 0) == 0
+    assert 0 < lib.la_decay_workspace_bytes(1, 4, 8192, 64, 64, 0) < lib.la_decay_workspace_bytes(1, 4, 8192, 64, 64, 1)
     for bad in ((0, 1, 64, 64, 64), (1, 1, 0, 64, 64), (1, 1, 8192, 129, 64), (1, 1, 8192, 64, 0), (1, -1, 8192, 64, 64)):
-        assert lib.la_decay_workspace_bytes(*bad) == 0
+        assert lib.la_decay_workspace_bytes(*bad, 0) == 0
 
 
 FWD = dict(q=P, k=P, v=P, dt=1, out=P, odt=1, B=1, H=2, N=8, d=16, dv=64, qs=None, ks=None, vs=None, g=P, lens=None,

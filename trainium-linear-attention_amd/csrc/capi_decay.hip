@@ -37,9 +37,9 @@ int operand(const void* p, const long long* s, int H, int N, int w, int esz, lon
 
 extern "C" {
 
-size_t la_decay_workspace_bytes(int B, int H, int N, int d, int dv) {
+size_t la_decay_workspace_bytes(int B, int H, int N, int d, int dv, int backward) {
   if (B < 1 || H < 1 || N < 1 || check_sizes(B, H, N, d, dv, 1.f) != LA_OK) return 0;
-  return la::decay_workspace_bytes((long long)B * H, N, d, dv);
+  return la::decay_workspace_bytes((long long)B * H, N, d, dv, backward != 0);
 }
 
 int la_decay_fwd(const void* q, const void* k, const void* v, int in_dtype, void* out, int out_dtype, int B, int H,
@@ -59,7 +59,7 @@ int la_decay_fwd(const void* q, const void* k, const void* v, int in_dtype, void
   if (!al(out, 16) || !al(log_decay, 4) || !al(lengths, 4) || !al(state_in, 16) || !al(state_out, 16))
     return LA_ERR_BAD_ALIGNMENT;
   if (overlap(state_in, state_out, (size_t)B * H * d * dv * 4)) return LA_ERR_OVERLAP;
-  const size_t need = la::decay_workspace_bytes((long long)B * H, N, d, dv);
+  const size_t need = la::decay_workspace_bytes((long long)B * H, N, d, dv, false);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return LA_ERR_WORKSPACE;
   if (need > 0 && !al(workspace, 16)) return LA_ERR_BAD_ALIGNMENT;
   a.q = q;
@@ -102,7 +102,7 @@ int la_decay_bwd(const void* q, const void* k, const void* v, const void* dout, 
       !al(dstate_out, 16) || !al(dstate_in, 16))
     return LA_ERR_BAD_ALIGNMENT;
   if (overlap(dstate_in, dstate_out, (size_t)B * H * d * dv * 4)) return LA_ERR_OVERLAP;
-  const size_t need = la::decay_workspace_bytes((long long)B * H, N, d, dv);
+  const size_t need = la::decay_workspace_bytes((long long)B * H, N, d, dv, true);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return LA_ERR_WORKSPACE;
   if (need > 0 && !al(workspace, 16)) return LA_ERR_BAD_ALIGNMENT;
   a.q = q;

@@ -15,8 +15,9 @@
 // once, their tiles dealt out to the waves, and go through LDS.
 //
 // Roundings for bf16 inputs: P and S enter bf16 products as two terms (16 bits), so that outputs are as
-// far from 64 bits as their own rounding; the weighted values enter the update as three (24 bits), so that
-// states, which are fp32, have fp32's accuracy.  fp32 inputs run on fp32 matrix instructions throughout.
+// far from 64 bits as their own rounding.  Weighted values enter the update as two as well, or as three (24 bits)
+// where the state is an output, which is fp32 and has fp32's accuracy.  fp32 inputs run on fp32 matrix
+// instructions throughout.
 #include <math.h>
 
 #include <algorithm>
@@ -29,17 +30,27 @@ namespace {
 
 constexpr int C = kDecayC;
 
-struct DecayParams {
+// One sum of the form above: its operands (in their roles), its states and its output.
+struct DecayJob {
   DecayTensor q, k, v;
   void* out;                   // contiguous (B, H, N, dv)
+  const float* state_in;       // (B, H, d, dv) or null; in_trans: (B, H, dv, d)
+  float* state_out;            // or null
+  float* seg;                  // segment states, DP DVP each, in accumulator order; null: one segment
+  float in_mul, out_mul;       // state_in is taken times in_mul, state_out written times out_mul
+  int d, dv;
+  int rev;                     // from the sequence's end
+  int in_trans, seg_trans;     // state_in, the segments' states are of the transposed state
+  int fine;                    // a state is an output: weighted values enter its updates in full
+};
+
+struct DecayParams {
   const float* log_decay;      // (H)
   const int* lengths;          // (B) or null: N
-  const float* state_in;       // (B, H, d, dv) or null; transposed: (B, H, dv, d)
-  float* state_out;            // or null
-  float* seg;                  // segment states (BH, nseg, DP * DVP) in accumulator order, or null: nseg = 1
-  int H, N, d, dv, nseg, seg_chunks;
-  float scale, in_mul, out_mul;   // state_in is taken times in_mul, state_out written times out_mul
-  int in_trans, out_f32;
+  int H, N, nseg, seg_chunks, units, njobs;   // units: (head, segment) pairs; work-groups: units njobs
+  float scale;
+  int out_f32;
+  DecayJob job[3];
 };
 
 __device__ __forceinline__ int seq_len(const DecayParams& p, int b) {
@@ -70,37 +81,75 @@ __device__ __forceinline__ size_t state_at(int d, int dv, size_t bh, int kd, int
   return trans ? (bh * dv + vd) * d + kd : (bh * d + kd) * dv + vd;
 }
 
-// Rows r0 .. r0 + 63 of a sequence of len tokens into an LDS tile of W columns; token of row r: r, or
-// len - 1 - r from the end.  Rows from len on and columns from w on are zero.
-template <bool F32, int W, int NT, bool REV>
-__device__ __forceinline__ void stage(const DecayTensor& x, size_t base, int w, int r0, int len,
-                                      typename DecayOps<F32>::elem* tile, int tid) {
-  typedef typename DecayOps<F32>::elem elem;
-  constexpr int LD = W + DecayOps<F32>::kPad, E = 16 / sizeof(elem), PIECES = W / E;
-  const elem* src = static_cast<const elem*>(x.p) + base;
-#pragma unroll
-  for (int i = 0; i < (C * PIECES + NT - 1) / NT; ++i) {
-    const int at = tid + NT * i;
-    if ((C * PIECES) % NT != 0 && at >= C * PIECES) break;
-    const int row = at / PIECES, col = at % PIECES * E, r = r0 + row;
-    u32x4 y = {0u, 0u, 0u, 0u};
-    if (r < len && col < w) {
-      const elem* s = src + (long long)(REV ? len - 1 - r : r) * x.s[2] + col;
-      if (x.vec) {
-        y = *reinterpret_cast<const u32x4*>(s);
-      } else {
-        elem e[E];
-#pragma unroll
-        for (int j = 0; j < E; ++j) e[j] = col + j < w ? s[j] : (elem)0;
-        y = __builtin_bit_cast(u32x4, e);
-      }
-    }
-    *reinterpret_cast<u32x4*>(tile + row * LD + col) = y;
+// A work-group's job and its (head, segment).  Work-groups go to the eight XCDs in turn: the jobs of one
+// (head, segment), which read the same tensors, are given to one XCD one after another, and meet in its L2.
+__device__ __forceinline__ int unit_of(const DecayParams& p, int& job) {
+  const int id = blockIdx.x;
+  if ((p.units & 7) == 0) {
+    const int slot = id >> 3;
+    job = slot % p.njobs;
+    return slot / p.njobs * 8 + (id & 7);
   }
+  job = id % p.njobs;
+  return id / p.njobs;
 }
 
+// Chunks of a (b, h)'s rows on their way to an LDS tile of W columns, in registers: row r of the sequence
+// is token r, or token len - 1 - r (rev).  VEC: rows are whole 16-byte pieces, read through a buffer over
+// the chunk's rows, so that rows behind the sequence and columns behind the row read as zeros without a branch.
+template <bool F32, int W, int NT, bool VEC>
+struct RowLoader {
+  typedef typename DecayOps<F32>::elem elem;
+  static constexpr int LD = W + DecayOps<F32>::kPad, E = 16 / sizeof(elem), PIECES = W / E, ALL = C * PIECES, NL = (ALL + NT - 1) / NT;
+  u32x4 x[NL];
+  int off[NL];
+  const elem* base;
+  long long row;        // elements between tokens
+  int w, rev;
+
+  __device__ __forceinline__ void init(const DecayTensor& t, int b, int h, int width, int reversed, int tid) {
+    base = static_cast<const elem*>(t.p) + b * t.s[0] + h * t.s[1];
+    row = t.s[2];
+    w = width;
+    rev = reversed;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int at = tid + NT * i, r = at / PIECES, col = at % PIECES * E;
+      off[i] = at < ALL && col < w ? (rev ? C - 1 - r : r) * (int)(row * sizeof(elem)) + col * (int)sizeof(elem) : kOffOutOfRange;
+    }
+  }
+  // rows r0 .. r0 + n - 1 (n <= 64) of len; the others zeros
+  __device__ __forceinline__ void load(int r0, int n, int len, int tid) {
+    if (VEC) {
+      // n >= 1: a last load past the end is of the last chunk again, and not used
+      const int rb = (int)(row * sizeof(elem));
+      const auto rs = make_rsrc(base + (rev ? len - r0 - n : r0) * row, (u32)((n - 1) * rb + w * (int)sizeof(elem)));
+      const int back = rev ? (C - n) * rb : 0;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) x[i] = buf_load_b128(rs, off[i] - back);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int at = tid + NT * i, r = at / PIECES, col = at % PIECES * E;
+        elem e[E];
+        const elem* s = base + (long long)(rev ? len - 1 - r0 - r : r0 + r) * row + col;
+#pragma unroll
+        for (int j = 0; j < E; ++j) e[j] = at < ALL && r < n && col + j < w ? s[j] : (elem)0;
+        x[i] = __builtin_bit_cast(u32x4, e);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(elem* tile, int tid) const {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int at = tid + NT * i;
+      if (ALL % NT == 0 || at < ALL) *reinterpret_cast<u32x4*>(tile + at / PIECES * LD + at % PIECES * E) = x[i];
+    }
+  }
+};
+
 // One segment.  OUT: outputs (and, with one segment, the last state); else the segment's own state.
-template <bool F32, int DP, int DVP, bool REV, bool OUT>
+template <bool F32, int DP, int DVP, bool OUT, bool VEC>
 __global__ __launch_bounds__(4 * DVP) void decay_kernel(const DecayParams p) {
   typedef DecayOps<F32> Ops;
   typedef typename Ops::elem elem;
@@ -111,16 +160,17 @@ __global__ __launch_bounds__(4 * DVP) void decay_kernel(const DecayParams p) {
   __shared__ __attribute__((aligned(16))) elem Ks[C * LDK];
   __shared__ __attribute__((aligned(16))) elem Vs[C * LDV];
   __shared__ __attribute__((aligned(16))) elem Ps[OUT ? NP * C * LDP : 1];
-  __shared__ float gq[C], gv[C];      // g^(i + 1) of the queries, g^(n - 1 - j) of a chunk's n keys
+  __shared__ __attribute__((aligned(16))) float gq[C], gv[C];      // g^(i + 1) of the queries, g^(n - 1 - j) of a chunk's n keys
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n16 = lane & 15, g = lane >> 4;
-  const int bh = blockIdx.x / p.nseg, seg = blockIdx.x - bh * p.nseg, b = bh / p.H, h = bh - b * p.H;
-  const int len = seq_len(p, b), d = p.d, dv = p.dv, N = p.N;
-  const int first = seg * p.seg_chunks * C, end = min(N, first + p.seg_chunks * C);
+  int jn;
+  const int unit = unit_of(p, jn), bh = unit / p.nseg, seg = unit - bh * p.nseg, b = bh / p.H, h = bh - b * p.H;
+  const DecayJob& job = p.job[jn];
+  const int len = seq_len(p, b), d = job.d, dv = job.dv, N = p.N, rev = job.rev;
+  const int first = seg * p.seg_chunks * C, end = min(N, first + p.seg_chunks * C), stop = min(end, len);
   const float lg = log2_decay(p, h);
-  const size_t qb = (size_t)(b * p.q.s[0] + h * p.q.s[1]), kb = (size_t)(b * p.k.s[0] + h * p.k.s[1]),
-               vb = (size_t)(b * p.v.s[0] + h * p.v.s[1]);
+  const int esz = p.out_f32 ? 4 : 2;
 
   // st[t][r] = S[16 t + 4 g + r][16 w + n16]
   f32x4 st[DT];
@@ -128,47 +178,68 @@ __global__ __launch_bounds__(4 * DVP) void decay_kernel(const DecayParams p) {
   for (int t = 0; t < DT; ++t) {
     st[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
     if (OUT) {
-      if (p.seg != nullptr) {
-        st[t] = *reinterpret_cast<const f32x4*>(p.seg + ((size_t)blockIdx.x * NW * DT + w * DT + t) * 256 + 4 * lane);
-      } else if (p.state_in != nullptr) {
+      if (job.seg != nullptr) {
+        const float* rec = job.seg + (size_t)unit * (DP * DVP);
+        if (job.seg_trans) {      // the record is of the transposed state
+#pragma unroll
+          for (int r = 0; r < 4; ++r) st[t][r] = rec[(t * NW + w) * 256 + (n16 >> 2) * 64 + (4 * g + r) * 4 + (n16 & 3)];
+        } else {
+          st[t] = *reinterpret_cast<const f32x4*>(rec + (w * DT + t) * 256 + 4 * lane);
+        }
+      } else if (job.state_in != nullptr) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int kd = 16 * t + 4 * g + r, vd = 16 * w + n16;
-          if (kd < d && vd < dv) st[t][r] = p.state_in[state_at(d, dv, bh, kd, vd, p.in_trans)] * p.in_mul;
+          if (kd < d && vd < dv) st[t][r] = job.state_in[state_at(d, dv, bh, kd, vd, job.in_trans)] * job.in_mul;
         }
       }
     }
   }
+  if (OUT) {      // rows behind the sequence
+    const size_t o = (size_t)bh * N * dv;
+    for (size_t i = (size_t)max(first, len) * dv + tid; i < (size_t)end * dv; i += NT) {
+      if (p.out_f32) static_cast<float*>(job.out)[o + i] = 0.f;
+      else static_cast<uint16_t*>(job.out)[o + i] = 0;
+    }
+  }
   const Fade whole(lg, C);
   if (tid < C) {
-    gq[tid] = exp2_raw(lg * (float)(tid + (REV ? 0 : 1)));
-    gv[tid] = exp2_raw(lg * (float)(C - 1 - tid + (REV ? 1 : 0)));
+    gq[tid] = exp2_raw(lg * (float)(tid + 1 - rev));
+    gv[tid] = exp2_raw(lg * (float)(C - 1 - tid + rev));
   }
   if (OUT)   // tiles above the diagonal that a step of 32 keys reads
     for (int i = tid; i < NP * 512; i += NT) {
       const int part = i >> 9, x = i & 511, tile = x >> 8, row = (x >> 4) & 15, col = x & 15;
       Ps[(part * C + 32 * tile + row) * LDP + 32 * tile + 16 + col] = (elem)0;
     }
+  const bool fine = NF > 1 && job.fine;
 
-  for (int r0 = first; r0 < end; r0 += C) {
-    const int n = min(C, len - r0);      // tokens of this chunk
-    if (n <= 0) {
-      if (!OUT) break;
-      for (int i = tid; i < C * dv; i += NT) {      // rows behind the sequence
-        const int row = r0 + i / dv;
-        if (row < N) {
-          const size_t o = ((size_t)bh * N + row) * dv + i % dv;
-          if (p.out_f32) static_cast<float*>(p.out)[o] = 0.f;
-          else static_cast<uint16_t*>(p.out)[o] = 0;
-        }
-      }
-      continue;
-    }
+  RowLoader<F32, DP, NT, VEC> ql, kl;
+  RowLoader<F32, DVP, NT, VEC> vl;
+  if (OUT) ql.init(job.q, b, h, d, rev, tid);
+  kl.init(job.k, b, h, d, rev, tid);
+  vl.init(job.v, b, h, dv, rev, tid);
+  if (first < stop) {
+    const int n = min(C, stop - first);
+    if (OUT) ql.load(first, n, len, tid);
+    kl.load(first, n, len, tid);
+    vl.load(first, n, len, tid);
+  }
+  const bool keep = !OUT || (job.seg == nullptr && job.state_out != nullptr);      // the last chunk's update counts
+
+  for (int r0 = first; r0 < stop; r0 += C) {
+    const int n = min(C, stop - r0);      // tokens of this chunk
     __syncthreads();
-    if (OUT) stage<F32, DP, NT, REV>(p.q, qb, d, r0, len, Qs, tid);
-    stage<F32, DP, NT, REV>(p.k, kb, d, r0, len, Ks, tid);
-    stage<F32, DVP, NT, REV>(p.v, vb, dv, r0, len, Vs, tid);
-    if (n < C && tid < C) gv[tid] = exp2_raw(lg * (float)max(n - 1 - tid + (REV ? 1 : 0), 0));
+    if (OUT) ql.store(Qs, tid);
+    kl.store(Ks, tid);
+    vl.store(Vs, tid);
+    if (n < C && tid < C) gv[tid] = exp2_raw(lg * (float)max(n - 1 - tid + rev, 0));
+    {      // the next chunk's rows, in flight while this one is computed
+      const int next = r0 + C < stop ? r0 + C : r0, m = min(C, stop - next);
+      if (OUT) ql.load(next, m, len, tid);
+      kl.load(next, m, len, tid);
+      vl.load(next, m, len, tid);
+    }
     __syncthreads();
     frag vf[2];
 #pragma unroll
@@ -205,6 +276,8 @@ __global__ __launch_bounds__(4 * DVP) void decay_kernel(const DecayParams p) {
       for (int x = 0; x < DP / 32; ++x)
         Ops::template parts<NP>({{st[2 * x][0], st[2 * x][1], st[2 * x][2], st[2 * x][3], st[2 * x + 1][0],
                                   st[2 * x + 1][1], st[2 * x + 1][2], st[2 * x + 1][3]}}, sp[x]);
+      // rows of the chunk in the output, from token r0 or, from the end, len - r0 - n
+      const auto orow = make_rsrc(static_cast<char*>(job.out) + ((size_t)bh * N + (rev ? len - r0 - n : r0)) * (dv * esz), (u32)(n * dv * esz));
 #pragma unroll
       for (int qt = 0; qt < 4; ++qt) {
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -222,32 +295,34 @@ __global__ __launch_bounds__(4 * DVP) void decay_kernel(const DecayParams p) {
           for (int part = 0; part < NP; ++part)
             o = Ops::mma(vf[s], Ops::row(Ps + (part * C + 16 * qt + n16) * LDP + 32 * s + 8 * g), o);
         o *= p.scale;
-        const int r = r0 + 16 * qt + n16, vd = 16 * w + 4 * g;
-        if (r < N && vd < dv) {
-          const int t = r < len ? (REV ? len - 1 - r : r) : r;
-          if (r >= len) o = (f32x4){0.f, 0.f, 0.f, 0.f};
-          const size_t at = ((size_t)bh * N + t) * dv + vd;
-          if ((dv & 3) == 0) {
-            if (p.out_f32) *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + at) = o;
-            else *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out) + at) = (u32x2){pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
-          } else {
+        const int r = 16 * qt + n16, vd = 16 * w + 4 * g, at = ((rev ? n - 1 - r : r) * dv + vd) * esz;
+        if ((dv & 3) == 0) {      // rows from n on are out of the buffer's range on either side
+          const int to = vd < dv ? at : kOffOutOfRange;
+          if (p.out_f32) buf_store_b128(__builtin_bit_cast(u32x4, o), orow, to);
+          else buf_store_b64((u32x2){pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])}, orow, to);
+        } else if (r < n) {
+          const size_t to = ((size_t)bh * N + (rev ? len - 1 - r0 - r : r0 + r)) * dv + vd;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (vd + e < dv) {
-                if (p.out_f32) static_cast<float*>(p.out)[at + e] = o[e];
-                else static_cast<uint16_t*>(p.out)[at + e] = f32_to_bf16_bits(o[e]);
-              }
-          }
+          for (int e = 0; e < 4; ++e)
+            if (vd + e < dv) {
+              if (p.out_f32) static_cast<float*>(job.out)[to + e] = o[e];
+              else static_cast<uint16_t*>(job.out)[to + e] = f32_to_bf16_bits(o[e]);
+            }
         }
       }
-      if (r0 + C >= end && (p.seg != nullptr || p.state_out == nullptr)) break;
+      if (r0 + C >= stop && !keep) break;
     }
     // S <- g^n S + K^T (weighted V)
     const Fade fade = n == C ? whole : Fade(lg, n);
+    if (fade.slow) {
 #pragma unroll
-    for (int t = 0; t < DT; ++t)
+      for (int t = 0; t < DT; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) st[t][r] = fade(st[t][r]);
+        for (int r = 0; r < 4; ++r) st[t][r] = __builtin_fmaf(st[t][r], fade.f, st[t][r]);
+    } else {
+#pragma unroll
+      for (int t = 0; t < DT; ++t) st[t] *= fade.f;
+    }
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       f32x8 x = Ops::widen(vf[s]);
@@ -255,162 +330,206 @@ __global__ __launch_bounds__(4 * DVP) void decay_kernel(const DecayParams p) {
       for (int e = 0; e < 8; ++e) x.v[e] *= gv[32 * s + 8 * g + e];
       frag vp[NF];
       Ops::template parts<NF>(x, vp);
+      frag kf[DT];
 #pragma unroll
-      for (int t = 0; t < DT; ++t) {
-        const frag kf = Ops::col(Ks, LDK, 32 * s, 16 * t, lane);
+      for (int t = 0; t < DT; ++t) kf[t] = Ops::col(Ks, LDK, 32 * s, 16 * t, lane);
+      if (fine) {
 #pragma unroll
-        for (int part = NF - 1; part >= 0; --part) st[t] = Ops::mma(kf, vp[part], st[t]);
+        for (int t = 0; t < DT; ++t) st[t] = Ops::mma(kf[t], vp[NF - 1], st[t]);
       }
+#pragma unroll
+      for (int part = NF > 1 ? NF - 2 : 0; part >= 0; --part)
+#pragma unroll
+        for (int t = 0; t < DT; ++t) st[t] = Ops::mma(kf[t], vp[part], st[t]);
     }
   }
   if (!OUT) {
 #pragma unroll
     for (int t = 0; t < DT; ++t)
-      *reinterpret_cast<f32x4*>(p.seg + ((size_t)blockIdx.x * NW * DT + w * DT + t) * 256 + 4 * lane) = st[t];
-  } else if (p.seg == nullptr && p.state_out != nullptr) {
+      *reinterpret_cast<f32x4*>(job.seg + ((size_t)unit * NW * DT + w * DT + t) * 256 + 4 * lane) = st[t];
+  } else if (job.seg == nullptr && job.state_out != nullptr) {
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int kd = 16 * t + 4 * g + r, vd = 16 * w + n16;
-        if (kd < d && vd < dv) p.state_out[state_at(d, dv, bh, kd, vd, 0)] = st[t][r] * p.out_mul;
+        if (kd < d && vd < dv) job.state_out[state_at(d, dv, bh, kd, vd, 0)] = st[t][r] * job.out_mul;
       }
   }
 }
 
-// Segments' own states to the states before them, in place, and the last state: one thread an entry of
-// one head, eight segments' loads in flight.
+// Segments' own states to the states before them, in place, and the last state: a thread has one entry of one
+// head, 16 segments' loads in flight.
+constexpr int kScanThreads = 64, kScanLoads = 16;
 template <int DP, int DVP>
-__global__ __launch_bounds__(256) void decay_scan_kernel(const DecayParams p) {
-  constexpr int REC = DP * DVP;
-  const int per = REC / 256, bh = blockIdx.x / per, e = (blockIdx.x - bh * per) * 256 + threadIdx.x;
-  const int b = bh / p.H, h = bh - b * p.H, len = seq_len(p, b);
+__global__ __launch_bounds__(kScanThreads) void decay_scan_kernel(const DecayParams p) {
+  constexpr int REC = DP * DVP, per = REC / kScanThreads;
+  const DecayJob& job = p.job[blockIdx.y];
+  const int bh = blockIdx.x / per, e = (blockIdx.x - bh * per) * kScanThreads + threadIdx.x;
+  const int b = bh / p.H, h = bh - b * p.H, len = seq_len(p, b), d = job.d, dv = job.dv;
   const int vec = e >> 8, lane = (e >> 2) & 63, kd = 16 * (vec % (DP / 16)) + 4 * (lane >> 4) + (e & 3),
             vd = 16 * (vec / (DP / 16)) + (lane & 15);
-  const bool real = kd < p.d && vd < p.dv;
+  const bool real = kd < d && vd < dv;
   const float lg = log2_decay(p, h);
   const int seg_tokens = p.seg_chunks * C;
   const Fade whole(lg, seg_tokens);
   float s = 0.f;
-  if (p.state_in != nullptr && real) s = p.state_in[state_at(p.d, p.dv, bh, kd, vd, p.in_trans)] * p.in_mul;
-  float* rec = p.seg + (size_t)bh * p.nseg * REC + e;
-  for (int i0 = 0; i0 < p.nseg; i0 += 8) {
-    float x[8];
+  if (job.state_in != nullptr && real) s = job.state_in[state_at(d, dv, bh, kd, vd, job.in_trans)] * job.in_mul;
+  float* rec = job.seg + (size_t)bh * p.nseg * REC + e;
+  for (int i0 = 0; i0 < p.nseg; i0 += kScanLoads) {
+    float x[kScanLoads];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = i0 + j < p.nseg ? rec[(size_t)(i0 + j) * REC] : 0.f;
+    for (int j = 0; j < kScanLoads; ++j) x[j] = i0 + j < p.nseg ? rec[(size_t)(i0 + j) * REC] : 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < kScanLoads; ++j) {
       if (i0 + j >= p.nseg) break;
       rec[(size_t)(i0 + j) * REC] = s;
       const int n = min(seg_tokens, max(0, len - (i0 + j) * seg_tokens));
       s = (n == seg_tokens ? whole : Fade(lg, n))(s) + x[j];
     }
   }
-  if (p.state_out != nullptr && real) p.state_out[state_at(p.d, p.dv, bh, kd, vd, 0)] = s * p.out_mul;
+  if (job.state_out != nullptr && real) job.state_out[state_at(d, dv, bh, kd, vd, 0)] = s * job.out_mul;
 }
 
 int pad_dim(int x) { return x <= 32 ? 32 : x <= 64 ? 64 : 128; }
 
-// Segments of a sequence: enough work-groups for the chip (four a CU), at least four chunks each.
+#ifndef LA_DECAY_WGS
+#define LA_DECAY_WGS 4      // work-groups a CU that sequences are cut for
+#endif
+
+// Segments of a sequence: enough work-groups for the chip, at least four chunks each.
 int segments(long long BH, int N) {
   const int chunks = (N + C - 1) / C;
-  const long long want = (4LL * device_cu_count() + BH - 1) / BH;
+  const long long want = ((long long)LA_DECAY_WGS * device_cu_count() + BH - 1) / BH;
   return (int)std::max(1LL, std::min(want, (long long)(chunks / 4)));
 }
 
-template <bool F32, int DP, int DVP, bool REV>
-int launch_pass(DecayParams p, int BH, hipStream_t stream) {
-  const dim3 grid((unsigned)(BH * p.nseg)), block(4 * DVP);
-  if (p.seg != nullptr) {
-    hipLaunchKernelGGL((decay_kernel<F32, DP, DVP, REV, false>), grid, block, 0, stream, p);
-    hipLaunchKernelGGL((decay_scan_kernel<DP, DVP>), dim3((unsigned)(BH * (DP * DVP / 256))), dim3(256), 0, stream, p);
-  }
-  hipLaunchKernelGGL((decay_kernel<F32, DP, DVP, REV, true>), grid, block, 0, stream, p);
-  return (int)hipGetLastError();
+enum Pass { kStates, kScan, kOutputs };
+
+template <bool F32, int DP, int DVP>
+void launch_dims(const DecayParams& p, Pass pass, hipStream_t stream) {
+  const dim3 grid((unsigned)(p.units * p.njobs)), block(4 * DVP);
+  bool vec = true;
+  for (int j = 0; j < p.njobs; ++j) vec = vec && p.job[j].k.vec && p.job[j].v.vec && (pass != kOutputs || p.job[j].q.vec);
+  if (pass == kScan)
+    hipLaunchKernelGGL((decay_scan_kernel<DP, DVP>), dim3((unsigned)(p.units / p.nseg * (DP * DVP / kScanThreads)), (unsigned)p.njobs),
+                       dim3(kScanThreads), 0, stream, p);
+  else if (pass == kStates && vec)
+    hipLaunchKernelGGL((decay_kernel<F32, DP, DVP, false, true>), grid, block, 0, stream, p);
+  else if (pass == kStates)
+    hipLaunchKernelGGL((decay_kernel<F32, DP, DVP, false, false>), grid, block, 0, stream, p);
+  else if (vec)
+    hipLaunchKernelGGL((decay_kernel<F32, DP, DVP, true, true>), grid, block, 0, stream, p);
+  else
+    hipLaunchKernelGGL((decay_kernel<F32, DP, DVP, true, false>), grid, block, 0, stream, p);
 }
 
-template <bool F32, bool REV>
-int launch_dims(const DecayParams& p, int BH, hipStream_t stream) {
-  const int dp = pad_dim(p.d), dvp = pad_dim(p.dv);
+// One pass over the first n of p's jobs, which have the same widths.
+template <bool F32>
+void launch_pass(DecayParams p, int n, Pass pass, hipStream_t stream) {
+  const int dp = pad_dim(p.job[0].d), dvp = pad_dim(p.job[0].dv);
+  p.njobs = n;
 #define LA_DECAY(DP, DVP) \
-  if (dp == DP && dvp == DVP) return launch_pass<F32, DP, DVP, REV>(p, BH, stream);
+  if (dp == DP && dvp == DVP) return launch_dims<F32, DP, DVP>(p, pass, stream);
   LA_DECAY(32, 32) LA_DECAY(32, 64) LA_DECAY(32, 128)
   LA_DECAY(64, 32) LA_DECAY(64, 64) LA_DECAY(64, 128)
   LA_DECAY(128, 32) LA_DECAY(128, 64) LA_DECAY(128, 128)
 #undef LA_DECAY
-  return (int)hipErrorInvalidValue;
 }
 
 DecayTensor operand(const void* ptr, const long long* s, int w, bool f32) {
   DecayTensor x{ptr, {s[0], s[1], s[2]}, 0};
   const int e = f32 ? 4 : 8;
-  x.vec = (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && w % e == 0 && s[0] % e == 0 && s[1] % e == 0 && s[2] % e == 0;
+  // 64 rows stay within 2^29 bytes, a buffer's offsets
+  x.vec = (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && w % e == 0 && s[0] % e == 0 && s[1] % e == 0 && s[2] % e == 0 &&
+          s[2] * (f32 ? 4 : 2) <= (1 << 23);
   return x;
 }
 
-int run_pass(const DecayParams& base, bool in_f32, bool rev, int BH, void* workspace, hipStream_t stream) {
-  DecayParams p = base;
-  p.nseg = segments(BH, p.N);
-  const int chunks = (p.N + C - 1) / C;
-  p.seg_chunks = (chunks + p.nseg - 1) / p.nseg;
+DecayParams common(const DecayArgs& a) {
+  DecayParams p{};
+  p.log_decay = a.log_decay;
+  p.lengths = a.lengths;
+  p.H = a.H;
+  p.N = a.N;
+  const int chunks = (a.N + C - 1) / C, nseg = segments((long long)a.B * a.H, a.N);
+  p.seg_chunks = (chunks + nseg - 1) / nseg;
   p.nseg = (chunks + p.seg_chunks - 1) / p.seg_chunks;
-  p.seg = p.nseg > 1 ? static_cast<float*>(workspace) : nullptr;
-  if (in_f32) return rev ? launch_dims<true, true>(p, BH, stream) : launch_dims<true, false>(p, BH, stream);
-  return rev ? launch_dims<false, true>(p, BH, stream) : launch_dims<false, false>(p, BH, stream);
+  p.units = a.B * a.H * p.nseg;
+  p.scale = a.scale;
+  return p;
 }
 
 }  // namespace
 
-size_t decay_workspace_bytes(long long BH, int N, int d, int dv) {
+size_t decay_workspace_bytes(long long BH, int N, int d, int dv, bool backward) {
   const int n = segments(BH, N);
-  return n > 1 ? (size_t)BH * n * pad_dim(d) * pad_dim(dv) * sizeof(float) : 0;
+  return n > 1 ? (size_t)BH * n * pad_dim(d) * pad_dim(dv) * sizeof(float) * (backward ? 2 : 1) : 0;
 }
 
 int launch_decay_fwd(const DecayArgs& a, hipStream_t stream) {
-  DecayParams p{};
-  p.q = operand(a.q, a.q_strides, a.d, a.in_f32);
-  p.k = operand(a.k, a.k_strides, a.d, a.in_f32);
-  p.v = operand(a.v, a.v_strides, a.dv, a.in_f32);
-  p.out = a.out;
-  p.log_decay = a.log_decay;
-  p.lengths = a.lengths;
-  p.state_in = a.state_in;
-  p.state_out = a.state_out;
-  p.H = a.H;
-  p.N = a.N;
-  p.d = a.d;
-  p.dv = a.dv;
-  p.scale = a.scale;
-  p.in_mul = p.out_mul = 1.f;
+  DecayParams p = common(a);
   p.out_f32 = a.out_f32;
-  return run_pass(p, a.in_f32, false, a.B * a.H, a.workspace, stream);
+  DecayJob& j = p.job[0];
+  j.q = operand(a.q, a.q_strides, a.d, a.in_f32);
+  j.k = operand(a.k, a.k_strides, a.d, a.in_f32);
+  j.v = operand(a.v, a.v_strides, a.dv, a.in_f32);
+  j.out = a.out;
+  j.state_in = a.state_in;
+  j.state_out = a.state_out;
+  j.seg = p.nseg > 1 ? static_cast<float*>(a.workspace) : nullptr;
+  j.in_mul = j.out_mul = 1.f;
+  j.d = a.d;
+  j.dv = a.dv;
+  j.fine = a.state_out != nullptr;
+  auto pass = a.in_f32 ? launch_pass<true> : launch_pass<false>;
+  if (j.seg != nullptr) {
+    pass(p, 1, kStates, stream);
+    pass(p, 1, kScan, stream);
+  }
+  pass(p, 1, kOutputs, stream);
+  return (int)hipGetLastError();
 }
 
+// dq is the forward sum of (dy, v, k) from S^T; dk and dv are sums from the sequence's end, of (v, dy, q) from
+// dS^T and of (k, q, dy) from dS, where dS (not scaled by s) enters divided by s.  Two passes compute the
+// states of the segments, S of (k, v) and dS of (q, dy), which the three outputs' pass shares.
 int launch_decay_bwd(const DecayArgs& a, hipStream_t stream) {
   const DecayTensor q = operand(a.q, a.q_strides, a.d, a.in_f32), k = operand(a.k, a.k_strides, a.d, a.in_f32),
                     v = operand(a.v, a.v_strides, a.dv, a.in_f32), dy = operand(a.dout, a.dout_strides, a.dv, a.in_f32);
-  DecayParams p{};
-  p.log_decay = a.log_decay;
-  p.lengths = a.lengths;
-  p.H = a.H;
-  p.N = a.N;
-  p.scale = a.scale;
+  DecayParams p = common(a);
   p.out_f32 = a.in_f32;
-  const int BH = a.B * a.H;
-  // dq: (dy, v, k), from S^T
-  p.q = dy, p.k = v, p.v = k, p.out = a.dq, p.d = a.dv, p.dv = a.d;
-  p.state_in = a.state_in, p.in_trans = 1, p.in_mul = p.out_mul = 1.f;
-  int rc = run_pass(p, a.in_f32, false, BH, a.workspace, stream);
-  if (rc != 0) return rc;
-  // dk: (v, dy, q) from the end, from dS^T (not scaled by s, so it enters divided by it)
-  p.q = v, p.k = dy, p.v = q, p.out = a.dk;
-  p.state_in = a.dstate_out, p.in_mul = 1.f / a.scale;
-  rc = run_pass(p, a.in_f32, true, BH, a.workspace, stream);
-  if (rc != 0) return rc;
-  // dv: (k, q, dy) from the end, from dS; its last state is the first state's gradient over s
-  p.q = k, p.k = q, p.v = dy, p.out = a.dv_out, p.d = a.d, p.dv = a.dv;
-  p.in_trans = 0, p.state_out = a.dstate_in, p.out_mul = a.scale;
-  return run_pass(p, a.in_f32, true, BH, a.workspace, stream);
+  auto pass = a.in_f32 ? launch_pass<true> : launch_pass<false>;
+  float *s = nullptr, *ds = nullptr;
+  if (p.nseg > 1) {
+    s = static_cast<float*>(a.workspace);
+    ds = s + (size_t)p.units * pad_dim(a.d) * pad_dim(a.dv);
+  }
+  DecayJob js{}, jd{};      // S, from the beginning, and dS, from the end
+  js.k = k, js.v = v, js.seg = s, js.state_in = a.state_in, js.in_mul = js.out_mul = 1.f, js.d = a.d, js.dv = a.dv;
+  jd.q = k, jd.k = q, jd.v = dy, jd.out = a.dv_out, jd.seg = ds, jd.state_in = a.dstate_out, jd.state_out = a.dstate_in;
+  jd.in_mul = 1.f / a.scale, jd.out_mul = a.scale, jd.d = a.d, jd.dv = a.dv, jd.rev = 1, jd.fine = a.dstate_in != nullptr;
+  if (p.nseg > 1) {
+    p.job[0] = js;
+    p.job[1] = jd;
+    pass(p, 2, kStates, stream);
+    pass(p, 2, kScan, stream);
+  }
+  DecayJob jq = js, jk = jd;
+  jq.q = dy, jq.k = v, jq.v = k, jq.out = a.dq, jq.d = a.dv, jq.dv = a.d, jq.seg_trans = jq.in_trans = 1;
+  jk.q = v, jk.k = dy, jk.v = q, jk.out = a.dk, jk.d = a.dv, jk.dv = a.d, jk.seg_trans = jk.in_trans = 1;
+  jk.state_out = nullptr, jk.fine = 0;
+  p.job[0] = jq;
+  p.job[1] = jk;
+  p.job[2] = jd;
+  if (pad_dim(a.d) == pad_dim(a.dv)) {
+    pass(p, 3, kOutputs, stream);
+  } else {
+    pass(p, 2, kOutputs, stream);
+    p.job[0] = jd;
+    pass(p, 1, kOutputs, stream);
+  }
+  return (int)hipGetLastError();
 }
 
 }  // namespace la

@@ -206,7 +206,7 @@ int device_cu_count();   // compute units of the current device (256 when the qu
 bool identity_shape(int d, int dv);
 size_t identity_workspace_bytes(int BH, int N, int d, int dv);
 int launch_identity(const IdentityArgs& a, hipStream_t stream);
-size_t decay_workspace_bytes(long long BH, int N, int d, int dv);
+size_t decay_workspace_bytes(long long BH, int N, int d, int dv, bool backward);
 int launch_decay_fwd(const DecayArgs& a, hipStream_t stream);
 int launch_decay_bwd(const DecayArgs& a, hipStream_t stream);
 int launch_decay_step(const DecayStepArgs& a, hipStream_t stream);

@@ -79,7 +79,7 @@ _SIGNATURES = {
                                                _c_size, _c_void]),
     "la_based_parallel_strided_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_void, _c_void,
                                                             _c_void]),
-    "la_decay_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int]),
+    "la_decay_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
     "la_decay_fwd": (_c_int, [_c_void, _c_void, _c_void, _c_int, _c_void, _c_int, _c_int, _c_int, _c_int, _c_int,
                               _c_int, _c_void, _c_void, _c_void, _c_void, _c_void, _c_float, _c_void, _c_void,
                               _c_void, _c_size, _c_void]),

@@ -58,8 +58,8 @@ def _check_state(state, like, shape, name):
         raise _lib.BasedLAError(f"{name} must be fp32 {shape}")
 
 
-def _workspace(L, b, h, t, d, dv, device):
-    n = int(L.la_decay_workspace_bytes(b, h, t, d, dv))
+def _workspace(L, b, h, t, d, dv, backward, device):
+    n = int(L.la_decay_workspace_bytes(b, h, t, d, dv, backward))
     return (torch.empty(n, dtype=torch.uint8, device=device) if n else None), n
 
 
@@ -75,7 +75,7 @@ def _forward(q, k, v, log_decay, lengths, scale, state_in, return_state, odt):
     if t == 0 and return_state:      # nothing is launched: no token changes the state
         state.zero_() if si is None else state.copy_(si)
     L = _lib.lib()
-    ws, ws_bytes = _workspace(L, b, h, t, d, dv, q.device)
+    ws, ws_bytes = _workspace(L, b, h, t, d, dv, 0, q.device)
     rc = L.la_decay_fwd(_lib.ptr(qc), _lib.ptr(kc), _lib.ptr(vc), _lib.dtype_code(cdt), _lib.ptr(out),
                         _lib.dtype_code(kdt), b, h, t, d, dv, _strides(qc), _strides(kc), _strides(vc),
                         _lib.ptr(log_decay), _lib.ptr(lengths), scale, _lib.ptr(si), _lib.ptr(state), _lib.ptr(ws),
@@ -114,7 +114,7 @@ class _DecayAttention(torch.autograd.Function):
         if t == 0 and want:
             dsi.zero_() if dso is None else dsi.copy_(dso)
         L = _lib.lib()
-        ws, ws_bytes = _workspace(L, b, h, t, d, dv, q.device)
+        ws, ws_bytes = _workspace(L, b, h, t, d, dv, 1, q.device)
         rc = L.la_decay_bwd(_lib.ptr(qc), _lib.ptr(kc), _lib.ptr(vc), _lib.ptr(dyc), _lib.dtype_code(cdt), _lib.ptr(dq),
                             _lib.ptr(dk), _lib.ptr(dvo), b, h, t, d, dv, _strides(qc), _strides(kc), _strides(vc),
                             _strides(dyc), _lib.ptr(log_decay), _lib.ptr(lengths), ctx.scale, _lib.ptr(si),
