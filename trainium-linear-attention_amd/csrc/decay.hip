@@ -48,6 +48,7 @@ struct DecayParams {
   const float* log_decay;      // (H)
   const int* lengths;          // (B) or null: N
   int H, N, nseg, seg_chunks, units, njobs;   // units: (head, segment) pairs; work-groups: units njobs
+  int join;                    // no scan: a segment adds up the states of those before it
   float scale;
   int out_f32;
   DecayJob job[3];
@@ -69,9 +70,14 @@ struct Fade {
   float f;
   bool slow;
   __device__ __forceinline__ Fade(float lg, int n) {
-    const float e = lg * 0.693147180559945309f * (float)n;
-    slow = e > -0.693f;
-    f = slow ? expm1f(e) : expf(e);
+    const float e = lg * (float)n, x = e * 0.693147180559945309f;
+    slow = e > -1.f;
+    // e^x - 1 by its series, whose tenth term is below 2^-27 of the first for |x| <= ln 2
+    float s = 1.f / 362880.f;
+    const float c[8] = {1.f / 40320.f, 1.f / 5040.f, 1.f / 720.f, 1.f / 120.f, 1.f / 24.f, 1.f / 6.f, 0.5f, 1.f};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s = __builtin_fmaf(s, x, c[i]);
+    f = slow ? s * x : exp2_raw(e);
   }
   __device__ __forceinline__ float operator()(float x) const { return __builtin_fmaf(x, f, slow ? x : 0.f); }
 };
@@ -94,73 +100,79 @@ __device__ __forceinline__ int unit_of(const DecayParams& p, int& job) {
   return id / p.njobs;
 }
 
-// Chunks of a (b, h)'s rows on their way to an LDS tile of W columns, in registers: row r of the sequence
-// is token r, or token len - 1 - r (rev).  VEC: rows are whole 16-byte pieces, read through a buffer over
-// the chunk's rows, so that rows behind the sequence and columns behind the row read as zeros without a branch.
+// Chunks of a (b, h)'s rows on their way to an LDS tile of W columns, in registers, one chunk of 64 rows after
+// another: row r of the sequence is token r, or token len - 1 - r (rev).  VEC: rows are whole 16-byte pieces, read through
+// a buffer over the chunk's rows, so that rows behind the sequence and columns behind the row read as zeros without a branch.
 template <bool F32, int W, int NT, bool VEC>
 struct RowLoader {
   typedef typename DecayOps<F32>::elem elem;
-  static constexpr int LD = W + DecayOps<F32>::kPad, E = 16 / sizeof(elem), PIECES = W / E, ALL = C * PIECES, NL = (ALL + NT - 1) / NT;
+  static constexpr int E = 16 / sizeof(elem), PIECES = W / E, ALL = C * PIECES, NL = (ALL + NT - 1) / NT;
+  static constexpr int RPP = NT / PIECES;      // rows between a thread's pieces, which have one column
+  static_assert(NT % PIECES == 0, "a column per thread");
   u32x4 x[NL];
-  int off[NL];
-  const elem* base;
+  int off;              // of the first piece, in bytes
+  int rb;               // bytes between tokens (VEC)
+  const elem* p;        // the next chunk's first row in memory, as if it had 64
   long long row;        // elements between tokens
-  int w, rev;
+  int w;
 
-  __device__ __forceinline__ void init(const DecayTensor& t, int b, int h, int width, int reversed, int tid) {
-    base = static_cast<const elem*>(t.p) + b * t.s[0] + h * t.s[1];
+  __device__ __forceinline__ void init(const DecayTensor& t, int b, int h, int width, int rev, int first, int len, int tid) {
     row = t.s[2];
     w = width;
-    rev = reversed;
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int at = tid + NT * i, r = at / PIECES, col = at % PIECES * E;
-      off[i] = at < ALL && col < w ? (rev ? C - 1 - r : r) * (int)(row * sizeof(elem)) + col * (int)sizeof(elem) : kOffOutOfRange;
-    }
+    rb = (int)(row * sizeof(elem));
+    p = static_cast<const elem*>(t.p) + b * t.s[0] + h * t.s[1] + (rev ? len - first - C : first) * row;
+    const int r = tid / PIECES, col = tid % PIECES * E;
+    off = r < C && col < w ? (rev ? C - 1 - r : r) * rb + col * (int)sizeof(elem) : kOffOutOfRange;
   }
-  // rows r0 .. r0 + n - 1 (n <= 64) of len; the others zeros
-  __device__ __forceinline__ void load(int r0, int n, int len, int tid) {
+  // the next chunk, of n >= 1 rows; the others zeros
+  __device__ __forceinline__ void load(int n, int rev, int tid) {
     if (VEC) {
-      // n >= 1: a last load past the end is of the last chunk again, and not used
-      const int rb = (int)(row * sizeof(elem));
-      const auto rs = make_rsrc(base + (rev ? len - r0 - n : r0) * row, (u32)((n - 1) * rb + w * (int)sizeof(elem)));
-      const int back = rev ? (C - n) * rb : 0;
+      // from the end, the n rows are the last of the 64: the buffer starts at them, and earlier ones have negative
+      // offsets, which are out of range too, as kOffOutOfRange stays with any of these steps
+      const int back = rev ? (C - n) * rb : 0, step = rev ? -RPP * rb : RPP * rb;
+      const auto rs = make_rsrc(reinterpret_cast<const char*>(p) + back, (u32)((n - 1) * rb + w * (int)sizeof(elem)));
 #pragma unroll
-      for (int i = 0; i < NL; ++i) x[i] = buf_load_b128(rs, off[i] - back);
+      for (int i = 0; i < NL; ++i) x[i] = buf_load_b128(rs, off + (i * step - back));
     } else {
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const int at = tid + NT * i, r = at / PIECES, col = at % PIECES * E;
+        const int r = tid / PIECES + RPP * i, col = tid % PIECES * E;
         elem e[E];
-        const elem* s = base + (long long)(rev ? len - 1 - r0 - r : r0 + r) * row + col;
+        const elem* s = p + (long long)(rev ? C - 1 - r : r) * row + col;
 #pragma unroll
-        for (int j = 0; j < E; ++j) e[j] = at < ALL && r < n && col + j < w ? s[j] : (elem)0;
+        for (int j = 0; j < E; ++j) e[j] = r < n && col + j < w ? s[j] : (elem)0;
         x[i] = __builtin_bit_cast(u32x4, e);
       }
     }
+    p += rev ? -C * row : C * row;
   }
   __device__ __forceinline__ void store(elem* tile, int tid) const {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int at = tid + NT * i;
-      if (ALL % NT == 0 || at < ALL) *reinterpret_cast<u32x4*>(tile + at / PIECES * LD + at % PIECES * E) = x[i];
+      const int r = tid / PIECES + RPP * i;
+      if (ALL % NT == 0 || r < C) *reinterpret_cast<u32x4*>(tile + DecayOps<F32>::template at<W>(r, tid % PIECES * E)) = x[i];
     }
   }
 };
 
+// Row of a state's accumulators: entry r of tile t in lane group g is feature 32 (t / 2) + 8 g + 4 (t % 2) + r, so that
+// tiles 2 x and 2 x + 1 together are a fragment of the features 32 x + 8 g .. + 7, the order of Q's and K's rows.
+__device__ __forceinline__ int state_row(int t, int g, int r) { return 32 * (t >> 1) + 8 * g + 4 * (t & 1) + r; }
+
 // One segment.  OUT: outputs (and, with one segment, the last state); else the segment's own state.
 template <bool F32, int DP, int DVP, bool OUT, bool VEC>
-__global__ __launch_bounds__(4 * DVP) void decay_kernel(const DecayParams p) {
+__global__ __launch_bounds__(4 * DVP) __attribute__((amdgpu_waves_per_eu(DP <= 64 && DVP <= 64 && VEC ? 3 : 1))) void decay_kernel(const DecayParams p) {
   typedef DecayOps<F32> Ops;
   typedef typename Ops::elem elem;
   typedef typename Ops::frag frag;
-  constexpr int NW = DVP / 16, NT = 64 * NW, DT = DP / 16;
-  constexpr int LDK = DP + Ops::kPad, LDV = DVP + Ops::kPad, LDP = C + Ops::kPad, NP = Ops::kPair, NF = Ops::kFine;
-  __shared__ __attribute__((aligned(16))) elem Qs[OUT ? C * LDK : 1];
-  __shared__ __attribute__((aligned(16))) elem Ks[C * LDK];
-  __shared__ __attribute__((aligned(16))) elem Vs[C * LDV];
-  __shared__ __attribute__((aligned(16))) elem Ps[OUT ? NP * C * LDP : 1];
-  __shared__ __attribute__((aligned(16))) float gq[C], gv[C];      // g^(i + 1) of the queries, g^(n - 1 - j) of a chunk's n keys
+  constexpr int NW = DVP / 16, NT = 64 * NW, DT = DP / 16, KS = DP / 32, NP = Ops::kPair, NF = Ops::kFine;
+  constexpr int KR = Ops::row_elems(DP), VR = Ops::row_elems(DVP), PR = Ops::row_elems(C), KT = C * KR, VT = C * VR, PT = C * PR;
+  constexpr int NB = OUT ? 1 : 2;      // tiles of K and V: without outputs there is one barrier a chunk, and two of each
+  constexpr int TPW = (10 + NW - 1) / NW;      // score tiles a wave
+  // one array, so that addresses in different tiles differ by constants: K, V, Q, P
+  constexpr int VS = NB * KT, QS = VS + NB * VT, PS = QS + (OUT ? KT : 0);
+  __shared__ __attribute__((aligned(16))) elem lds[PS + (OUT ? NP * PT : 0)];
+  __shared__ __attribute__((aligned(16))) float gv[NB][C];      // g^(n - 1 - j) of a chunk's n keys
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n16 = lane & 15, g = lane >> 4;
@@ -169,100 +181,176 @@ __global__ __launch_bounds__(4 * DVP) void decay_kernel(const DecayParams p) {
   const DecayJob& job = p.job[jn];
   const int len = seq_len(p, b), d = job.d, dv = job.dv, N = p.N, rev = job.rev;
   const int first = seg * p.seg_chunks * C, end = min(N, first + p.seg_chunks * C), stop = min(end, len);
-  const float lg = log2_decay(p, h);
   const int esz = p.out_f32 ? 4 : 2;
 
-  // st[t][r] = S[16 t + 4 g + r][16 w + n16]
+  RowLoader<F32, DP, NT, VEC> ql, kl;
+  RowLoader<F32, DVP, NT, VEC> vl;
+  if (OUT) ql.init(job.q, b, h, d, rev, first, len, tid);
+  kl.init(job.k, b, h, d, rev, first, len, tid);
+  vl.init(job.v, b, h, dv, rev, first, len, tid);
+  // the rows of the chunk at r0 on their way
+  auto load = [&](int r0) {
+    if (r0 >= stop) return;
+    const int n = min(C, stop - r0);
+    if (OUT) ql.load(n, rev, tid);
+    kl.load(n, rev, tid);
+    vl.load(n, rev, tid);
+  };
+  load(first);
+  const float lg = log2_decay(p, h);
+  // .. and in the tiles, with the weights of its keys
+  auto put = [&](int r0, int buf) {
+    if (OUT) ql.store(lds + QS, tid);
+    kl.store(lds + buf * KT, tid);
+    vl.store(lds + VS + buf * VT, tid);
+    if (tid < C) gv[buf][tid] = exp2_raw(lg * (float)max(min(C, stop - r0) - 1 - tid + rev, 0));
+  };
+
+  // st[t][r] = S[state_row(t, g, r)][16 w + n16]
   f32x4 st[DT];
 #pragma unroll
-  for (int t = 0; t < DT; ++t) {
-    st[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    if (OUT) {
-      if (job.seg != nullptr) {
-        const float* rec = job.seg + (size_t)unit * (DP * DVP);
-        if (job.seg_trans) {      // the record is of the transposed state
+  for (int t = 0; t < DT; ++t) st[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  const int vd = 16 * w + n16;
+  if (OUT && job.state_in != nullptr && (job.seg == nullptr || p.join)) {
+    const auto rs = make_rsrc(job.state_in + (size_t)bh * d * dv, (u32)(d * dv * 4));
+    const int kstep = (job.in_trans ? 1 : dv) * 4, vat = vd < dv ? vd * (job.in_trans ? d : 1) * 4 : kOffOutOfRange;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) st[t][r] = rec[(t * NW + w) * 256 + (n16 >> 2) * 64 + (4 * g + r) * 4 + (n16 & 3)];
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int kd = state_row(t, g, r);
+        st[t][r] = job.in_mul * __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, kd < d ? vat + kd * kstep : kOffOutOfRange, 0, 0));
+      }
+  }
+  if (OUT && job.seg != nullptr) {
+    // The record of a segment, or of its transposed state: that one's wave and lane of our row r = 0
+    const int rt = state_row(0, g, 0), ttv = 2 * (vd >> 5) + (vd >> 2 & 1), gtv = vd >> 3 & 3;
+    const int at0 = job.seg_trans ? ((rt >> 4) * NW + ttv) * 256 + (16 * gtv + (rt & 15)) * 4 + (vd & 3) : w * DT * 256 + 4 * lane;
+    auto record = [&](const float* rec, f32x4 (&x)[DT]) {
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+        if (job.seg_trans) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[t][r] = rec[at0 + (t >> 1) * 2 * NW * 256 + (4 * (t & 1) + r) * 4];
         } else {
-          st[t] = *reinterpret_cast<const f32x4*>(rec + (w * DT + t) * 256 + 4 * lane);
+          x[t] = *reinterpret_cast<const f32x4*>(rec + at0 + t * 256);
         }
-      } else if (job.state_in != nullptr) {
+      }
+    };
+    if (!p.join) {
+      record(job.seg + (size_t)unit * (DP * DVP), st);
+    } else {
+      // the states of the segments before this one (whole ones, or this one is empty), a few in flight
+      constexpr int FLY = DT <= 2 ? 8 : DT <= 4 ? 4 : 1;
+      const Fade skip(lg, p.seg_chunks * C);
+      const float* rec = job.seg + (size_t)bh * p.nseg * (DP * DVP);
+      for (int i = 0; i < seg; i += FLY) {
+        f32x4 x[FLY][DT];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int kd = 16 * t + 4 * g + r, vd = 16 * w + n16;
-          if (kd < d && vd < dv) st[t][r] = job.state_in[state_at(d, dv, bh, kd, vd, job.in_trans)] * job.in_mul;
-        }
+        for (int j = 0; j < FLY; ++j)
+          if (i + j < seg) record(rec + (size_t)(i + j) * (DP * DVP), x[j]);
+#pragma unroll
+        for (int j = 0; j < FLY; ++j)
+          if (i + j < seg) {
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) st[t][r] = skip(st[t][r]) + x[j][t][r];
+          }
       }
     }
   }
-  if (OUT) {      // rows behind the sequence
+  if (OUT && len < end) {      // rows behind the sequence
     const size_t o = (size_t)bh * N * dv;
+#pragma unroll 1
     for (size_t i = (size_t)max(first, len) * dv + tid; i < (size_t)end * dv; i += NT) {
       if (p.out_f32) static_cast<float*>(job.out)[o + i] = 0.f;
       else static_cast<uint16_t*>(job.out)[o + i] = 0;
     }
   }
-  const Fade whole(lg, C);
-  if (tid < C) {
-    gq[tid] = exp2_raw(lg * (float)(tid + 1 - rev));
-    gv[tid] = exp2_raw(lg * (float)(C - 1 - tid + rev));
+  // Score tiles (queries 16 qt.., keys 16 kt..), kt <= qt, are dealt out to the waves; a wave too many repeats the last
+  // one.  sd: s g^(i - j) of this lane's places (one query, four keys), 0 above the diagonal.
+  auto tile_q = [](int t) { return t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3; };
+  f32x4 sd[TPW];
+  float gq[4];      // s g^(i + 1) of this lane's query of each tile
+#pragma unroll
+  for (int i = 0; i < TPW; ++i) {
+    const int t = min(w + NW * i, 9), qt = tile_q(t), kt = t - qt * (qt + 1) / 2, gap = 16 * (qt - kt) + n16 - 4 * g;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sd[i][r] = gap - r >= 0 ? p.scale * exp2_raw(lg * (float)(gap - r)) : 0.f;
   }
+#pragma unroll
+  for (int t = 0; t < 4; ++t) gq[t] = p.scale * exp2_raw(lg * (float)(16 * t + n16 + 1 - rev));
   if (OUT)   // tiles above the diagonal that a step of 32 keys reads
     for (int i = tid; i < NP * 512; i += NT) {
       const int part = i >> 9, x = i & 511, tile = x >> 8, row = (x >> 4) & 15, col = x & 15;
-      Ps[(part * C + 32 * tile + row) * LDP + 32 * tile + 16 + col] = (elem)0;
+      lds[PS + part * PT + Ops::template at<C>(32 * tile + row, 32 * tile + 16 + col)] = (elem)0;
     }
-  const bool fine = NF > 1 && job.fine;
-
-  RowLoader<F32, DP, NT, VEC> ql, kl;
-  RowLoader<F32, DVP, NT, VEC> vl;
-  if (OUT) ql.init(job.q, b, h, d, rev, tid);
-  kl.init(job.k, b, h, d, rev, tid);
-  vl.init(job.v, b, h, dv, rev, tid);
-  if (first < stop) {
-    const int n = min(C, stop - first);
-    if (OUT) ql.load(first, n, len, tid);
-    kl.load(first, n, len, tid);
-    vl.load(first, n, len, tid);
+  // this lane's places in a tile: row n16 of Q, K and of P, columns of K and of V
+  int krow[KS], prow[2], kcol[KS][2], vcol[2];
+#pragma unroll
+  for (int x = 0; x < KS; ++x) {
+    krow[x] = Ops::template at<DP>(n16, 32 * x + 8 * g);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) kcol[x][i] = Ops::template col_at<DP, 8>(i, 32 * x, lane);
   }
-  const bool keep = !OUT || (job.seg == nullptr && job.state_out != nullptr);      // the last chunk's update counts
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    prow[i] = PS + Ops::template at<C>(n16, 32 * i + 8 * g);
+    vcol[i] = VS + Ops::template col_at<DVP, 4>(i, 16 * w, lane);
+  }
+  // and in the output's rows of a chunk, in bytes, of its first tile
+  const int ob = dv * esz, vd0 = 16 * w + 4 * g;
+  const int oat = vd0 < dv ? (rev ? C - 1 - n16 : n16) * ob + vd0 * esz : kOffOutOfRange;
+  const bool fine = NF > 2 && job.fine;
+  // with one segment, or no scan, the last state is that of the last segment's work-group
+  const bool last = OUT && job.state_out != nullptr && (job.seg == nullptr || (p.join && (stop == len && (first < stop || seg == 0))));
+  const bool keep = !OUT || last;      // the last chunk's update counts
+  const Fade whole(lg, C);
 
+  if (first < stop) {
+    put(first, 0);
+    load(first + C);
+  }
+  int buf = 0;
   for (int r0 = first; r0 < stop; r0 += C) {
     const int n = min(C, stop - r0);      // tokens of this chunk
-    __syncthreads();
-    if (OUT) ql.store(Qs, tid);
-    kl.store(Ks, tid);
-    vl.store(Vs, tid);
-    if (n < C && tid < C) gv[tid] = exp2_raw(lg * (float)max(n - 1 - tid + rev, 0));
-    {      // the next chunk's rows, in flight while this one is computed
-      const int next = r0 + C < stop ? r0 + C : r0, m = min(C, stop - next);
-      if (OUT) ql.load(next, m, len, tid);
-      kl.load(next, m, len, tid);
-      vl.load(next, m, len, tid);
+    int w0 = w;
+    asm volatile("" : "+s"(w0));      // addresses of score tiles are computed anew: their registers would cost a work-group a CU
+    lds_barrier();      // tiles are whole, and the last chunk's P has been read
+    const elem *kt_ = lds + buf * KT, *vt_ = lds + buf * VT;
+    if (!OUT && r0 + C < stop) {      // the other tiles have been read
+      put(r0 + C, buf ^ 1);
+      load(r0 + 2 * C);
     }
-    __syncthreads();
     frag vf[2];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) vf[s] = Ops::col(Vs, LDV, 32 * s, 16 * w, lane);
+    for (int s = 0; s < 2; ++s) vf[s] = Ops::template col<DVP>(vt_ + vcol[0] + 32 * s * VR, vt_ + vcol[1] + 32 * s * VR);
+    f32x4 o[4];
     if (OUT) {
-      // scores: tiles (queries 16 qt.., keys 16 kt..), kt <= qt; a lane has one query and four keys
-      for (int t = w; t < 10; t += NW) {
-        const int qt = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, kt = t - qt * (qt + 1) / 2;
-        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+      f32x4 sc[TPW];
 #pragma unroll
-        for (int x = 0; x < DP / 32; ++x)
-          s = Ops::mma(Ops::row(Ks + (16 * kt + n16) * LDK + 32 * x + 8 * g), Ops::row(Qs + (16 * qt + n16) * LDK + 32 * x + 8 * g), s);
-        const int gap = 16 * (qt - kt) + n16 - 4 * g;
+      for (int i = 0; i < TPW; ++i) {
+        const int t = min(w0 + NW * i, 9), qt = tile_q(t), kt = t - qt * (qt + 1) / 2;
+        sc[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[r] = gap - r >= 0 ? s[r] * exp2_raw(lg * (float)(gap - r)) : 0.f;
-        elem* dst = Ps + (16 * qt + n16) * LDP + 16 * kt + 4 * g;
+        for (int x = 0; x < KS; ++x)
+          sc[i] = Ops::mma(Ops::row(kt_ + 16 * kt * KR + krow[x]), Ops::row(lds + QS + 16 * qt * KR + krow[x]), sc[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < TPW; ++i) {
+        const int t = min(w0 + NW * i, 9), qt = tile_q(t), kt = t - qt * (qt + 1) / 2;
+        f32x4 s;      // a score above the diagonal may be infinite
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[r] = sd[i][r] != 0.f ? sc[i][r] * sd[i][r] : 0.f;
+        elem* dst = lds + PS + 16 * qt * PR + Ops::template at<C>(n16, 16 * kt + 4 * g);
         if constexpr (F32) {
           *reinterpret_cast<f32x4*>(dst) = s;
         } else {
 #pragma unroll
           for (int part = 0; part < NP; ++part) {
             const u32x2 y = {pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3])};
-            *reinterpret_cast<u32x2*>(dst + part * C * LDP) = y;
+            *reinterpret_cast<u32x2*>(dst + part * PT) = y;
             s[0] -= bf16_lo_to_f32(y[0]);
             s[1] -= bf16_hi_to_f32(y[0]);
             s[2] -= bf16_lo_to_f32(y[1]);
@@ -270,91 +358,119 @@ __global__ __launch_bounds__(4 * DVP) void decay_kernel(const DecayParams p) {
           }
         }
       }
-      __syncthreads();
-      frag sp[DP / 32][NP];
+      __builtin_amdgcn_sched_barrier(0);      // phases kept apart: their operands together would not fit the registers
+      // earlier tokens
 #pragma unroll
-      for (int x = 0; x < DP / 32; ++x)
-        Ops::template parts<NP>({{st[2 * x][0], st[2 * x][1], st[2 * x][2], st[2 * x][3], st[2 * x + 1][0],
-                                  st[2 * x + 1][1], st[2 * x + 1][2], st[2 * x + 1][3]}}, sp[x]);
-      // rows of the chunk in the output, from token r0 or, from the end, len - r0 - n
-      const auto orow = make_rsrc(static_cast<char*>(job.out) + ((size_t)bh * N + (rev ? len - r0 - n : r0)) * (dv * esz), (u32)(n * dv * esz));
+      for (int qt = 0; qt < 4; ++qt) o[qt] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int qt = 0; qt < 4; ++qt) {
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        const elem* qrow = Qs + (16 * qt + n16) * LDK + 4 * g;
+      for (int x = 0; x < KS; ++x) {
+        const f32x4 a = st[2 * x], e = st[2 * x + 1];
+        frag sp[NP];
+        Ops::template parts<NP>({{a[0], a[1], a[2], a[3], e[0], e[1], e[2], e[3]}}, sp);
 #pragma unroll
-        for (int x = 0; x < DP / 32; ++x) {
-          const frag qf = Ops::rows4(qrow + 32 * x, qrow + 32 * x + 16);
+        for (int qt = 0; qt < 4; ++qt) {
+          const frag qf = Ops::row(lds + QS + 16 * qt * KR + krow[x]);
 #pragma unroll
-          for (int part = 0; part < NP; ++part) o = Ops::mma(sp[x][part], qf, o);
+          for (int part = 0; part < NP; ++part) o[qt] = Ops::mma(sp[part], qf, o[qt]);
         }
-        o *= gq[16 * qt + n16];
+      }
+#pragma unroll
+      for (int qt = 0; qt < 4; ++qt) o[qt] *= gq[qt];
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (keep || r0 + C < stop) {      // S <- g^n S + K^T (weighted V)
+      const Fade fade = n == C ? whole : Fade(lg, n);
+      if (fade.slow) {
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) st[t][r] = __builtin_fmaf(st[t][r], fade.f, st[t][r]);
+      } else {
+#pragma unroll
+        for (int t = 0; t < DT; ++t) st[t] *= fade.f;
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        f32x8 x = Ops::widen(vf[s]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x.v[e] *= gv[buf][32 * s + 8 * g + e];
+        auto kfrag = [&](int t) {
+          const int at = 4 * (t & 1) + 32 * s * KR;
+          return Ops::template col<DP>(kt_ + kcol[t / 2][0] + at, kt_ + kcol[t / 2][1] + at);
+        };
+        if (fine) {      // all parts, the least first
+          frag vp[NF];
+          Ops::template parts<NF>(x, vp);
+#pragma unroll
+          for (int t = 0; t < DT; ++t) {
+            const frag kf = kfrag(t);
+#pragma unroll
+            for (int part = NF - 1; part >= 0; --part) st[t] = Ops::mma(kf, vp[part], st[t]);
+          }
+        } else {
+          frag vp[NP];
+          Ops::template parts<NP>(x, vp);
+#pragma unroll
+          for (int t = 0; t < DT; ++t) {
+            const frag kf = kfrag(t);
+#pragma unroll
+            for (int part = NP - 1; part >= 0; --part) st[t] = Ops::mma(kf, vp[part], st[t]);
+          }
+        }
+      }
+    }
+    if (OUT) {
+      lds_barrier();      // P is whole, and the tiles have been read
+      if (r0 + C < stop) {
+        put(r0 + C, 0);
+        load(r0 + 2 * C);
+      }
+#pragma unroll
+      for (int qt = 0; qt < 4; ++qt)
 #pragma unroll
         for (int s = 0; s <= qt / 2; ++s)
 #pragma unroll
-          for (int part = 0; part < NP; ++part)
-            o = Ops::mma(vf[s], Ops::row(Ps + (part * C + 16 * qt + n16) * LDP + 32 * s + 8 * g), o);
-        o *= p.scale;
-        const int r = 16 * qt + n16, vd = 16 * w + 4 * g, at = ((rev ? n - 1 - r : r) * dv + vd) * esz;
-        if ((dv & 3) == 0) {      // rows from n on are out of the buffer's range on either side
-          const int to = vd < dv ? at : kOffOutOfRange;
-          if (p.out_f32) buf_store_b128(__builtin_bit_cast(u32x4, o), orow, to);
-          else buf_store_b64((u32x2){pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])}, orow, to);
-        } else if (r < n) {
-          const size_t to = ((size_t)bh * N + (rev ? len - 1 - r0 - r : r0 + r)) * dv + vd;
+          for (int part = 0; part < NP; ++part) o[qt] = Ops::mma(vf[s], Ops::row(lds + prow[s] + part * PT + 16 * qt * PR), o[qt]);
+      // Rows of the chunk in the output, from token r0 or, from the end, len - r0 - n; the others are out of the buffer's
+      // range on either side.
+      char* out = static_cast<char*>(job.out) + ((size_t)bh * N + (rev ? len - r0 - n : r0)) * ob;
+      if ((dv & 3) == 0) {
+        const auto orow = make_rsrc(out, (u32)(n * ob));
+        const int back = rev ? (C - n) * ob : 0, step = rev ? -16 * ob : 16 * ob;
+#pragma unroll
+        for (int qt = 0; qt < 4; ++qt) {
+          const int to = oat + (qt * step - back);
+          if (p.out_f32) buf_store_b128(__builtin_bit_cast(u32x4, o[qt]), orow, to);
+          else buf_store_b64((u32x2){pack_bf16x2(o[qt][0], o[qt][1]), pack_bf16x2(o[qt][2], o[qt][3])}, orow, to);
+        }
+      } else {
+#pragma unroll
+        for (int qt = 0; qt < 4; ++qt) {
+          const int r = 16 * qt + n16, at = (rev ? n - 1 - r : r) * dv + vd0;
+          if (r >= n) continue;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (vd + e < dv) {
-              if (p.out_f32) static_cast<float*>(job.out)[to + e] = o[e];
-              else static_cast<uint16_t*>(job.out)[to + e] = f32_to_bf16_bits(o[e]);
+            if (vd0 + e < dv) {
+              if (p.out_f32) reinterpret_cast<float*>(out)[at + e] = o[qt][e];
+              else reinterpret_cast<uint16_t*>(out)[at + e] = f32_to_bf16_bits(o[qt][e]);
             }
         }
       }
-      if (r0 + C >= stop && !keep) break;
-    }
-    // S <- g^n S + K^T (weighted V)
-    const Fade fade = n == C ? whole : Fade(lg, n);
-    if (fade.slow) {
-#pragma unroll
-      for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) st[t][r] = __builtin_fmaf(st[t][r], fade.f, st[t][r]);
     } else {
-#pragma unroll
-      for (int t = 0; t < DT; ++t) st[t] *= fade.f;
-    }
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      f32x8 x = Ops::widen(vf[s]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x.v[e] *= gv[32 * s + 8 * g + e];
-      frag vp[NF];
-      Ops::template parts<NF>(x, vp);
-      frag kf[DT];
-#pragma unroll
-      for (int t = 0; t < DT; ++t) kf[t] = Ops::col(Ks, LDK, 32 * s, 16 * t, lane);
-      if (fine) {
-#pragma unroll
-        for (int t = 0; t < DT; ++t) st[t] = Ops::mma(kf[t], vp[NF - 1], st[t]);
-      }
-#pragma unroll
-      for (int part = NF > 1 ? NF - 2 : 0; part >= 0; --part)
-#pragma unroll
-        for (int t = 0; t < DT; ++t) st[t] = Ops::mma(kf[t], vp[part], st[t]);
+      buf ^= 1;
     }
   }
-  if (!OUT) {
 #pragma unroll
-    for (int t = 0; t < DT; ++t)
+  for (int t = 0; t < DT; ++t) {
+    if (!OUT) {
       *reinterpret_cast<f32x4*>(job.seg + ((size_t)unit * NW * DT + w * DT + t) * 256 + 4 * lane) = st[t];
-  } else if (job.seg == nullptr && job.state_out != nullptr) {
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
+    } else if (last) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int kd = 16 * t + 4 * g + r, vd = 16 * w + n16;
+        const int kd = state_row(t, g, r);
         if (kd < d && vd < dv) job.state_out[state_at(d, dv, bh, kd, vd, 0)] = st[t][r] * job.out_mul;
       }
+    }
   }
 }
 
@@ -367,7 +483,7 @@ __global__ __launch_bounds__(kScanThreads) void decay_scan_kernel(const DecayPar
   const DecayJob& job = p.job[blockIdx.y];
   const int bh = blockIdx.x / per, e = (blockIdx.x - bh * per) * kScanThreads + threadIdx.x;
   const int b = bh / p.H, h = bh - b * p.H, len = seq_len(p, b), d = job.d, dv = job.dv;
-  const int vec = e >> 8, lane = (e >> 2) & 63, kd = 16 * (vec % (DP / 16)) + 4 * (lane >> 4) + (e & 3),
+  const int vec = e >> 8, lane = (e >> 2) & 63, kd = state_row(vec % (DP / 16), lane >> 4, e & 3),
             vd = 16 * (vec / (DP / 16)) + (lane & 15);
   const bool real = kd < d && vd < dv;
   const float lg = log2_decay(p, h);
@@ -394,14 +510,29 @@ __global__ __launch_bounds__(kScanThreads) void decay_scan_kernel(const DecayPar
 int pad_dim(int x) { return x <= 32 ? 32 : x <= 64 ? 64 : 128; }
 
 #ifndef LA_DECAY_WGS
-#define LA_DECAY_WGS 4      // work-groups a CU that sequences are cut for
+#define LA_DECAY_WGS 3      // work-groups a CU that sequences are cut for
+#endif
+#ifndef LA_DECAY_JOIN
+#define LA_DECAY_JOIN 131072
 #endif
 
-// Segments of a sequence: enough work-groups for the chip, at least four chunks each.
-int segments(long long BH, int N) {
-  const int chunks = (N + C - 1) / C;
-  const long long want = ((long long)LA_DECAY_WGS * device_cu_count() + BH - 1) / BH;
-  return (int)std::max(1LL, std::min(want, (long long)(chunks / 4)));
+// Segments of a sequence: enough work-groups for the chip, of at least four chunks; two where the states of a head's
+// segments are so few bytes that each segment adds up those before it, without a scan.
+struct Segments {
+  int n, chunks;
+  bool join;
+};
+Segments segments(long long BH, int N, int d, int dv) {
+  const int chunks = (N + C - 1) / C, few = LA_DECAY_JOIN / (pad_dim(d) * pad_dim(dv) * (int)sizeof(float));
+  const long long want = (long long)LA_DECAY_WGS * device_cu_count() / BH;
+  long long n = std::min(want, (long long)(chunks / 4));
+  if (n < few) n = std::min({want, (long long)(chunks / 2), (long long)few});
+  n = std::max(1LL, n);
+  Segments s{};
+  s.chunks = (int)((chunks + n - 1) / n);
+  s.n = (chunks + s.chunks - 1) / s.chunks;
+  s.join = s.n > 1 && s.n <= few;
+  return s;
 }
 
 enum Pass { kStates, kScan, kOutputs };
@@ -440,9 +571,9 @@ void launch_pass(DecayParams p, int n, Pass pass, hipStream_t stream) {
 DecayTensor operand(const void* ptr, const long long* s, int w, bool f32) {
   DecayTensor x{ptr, {s[0], s[1], s[2]}, 0};
   const int e = f32 ? 4 : 8;
-  // 64 rows stay within 2^29 bytes, a buffer's offsets
+  // rows that do not overlap, 64 of them within 2^29 bytes: a buffer's offsets tell rows behind a sequence by their size
   x.vec = (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && w % e == 0 && s[0] % e == 0 && s[1] % e == 0 && s[2] % e == 0 &&
-          s[2] * (f32 ? 4 : 2) <= (1 << 23);
+          s[2] >= w && s[2] * (f32 ? 4 : 2) <= (1 << 23);
   return x;
 }
 
@@ -452,9 +583,10 @@ DecayParams common(const DecayArgs& a) {
   p.lengths = a.lengths;
   p.H = a.H;
   p.N = a.N;
-  const int chunks = (a.N + C - 1) / C, nseg = segments((long long)a.B * a.H, a.N);
-  p.seg_chunks = (chunks + nseg - 1) / nseg;
-  p.nseg = (chunks + p.seg_chunks - 1) / p.seg_chunks;
+  const Segments s = segments((long long)a.B * a.H, a.N, a.d, a.dv);
+  p.seg_chunks = s.chunks;
+  p.nseg = s.n;
+  p.join = s.join;
   p.units = a.B * a.H * p.nseg;
   p.scale = a.scale;
   return p;
@@ -463,7 +595,7 @@ DecayParams common(const DecayArgs& a) {
 }  // namespace
 
 size_t decay_workspace_bytes(long long BH, int N, int d, int dv, bool backward) {
-  const int n = segments(BH, N);
+  const int n = segments(BH, N, d, dv).n;
   return n > 1 ? (size_t)BH * n * pad_dim(d) * pad_dim(dv) * sizeof(float) * (backward ? 2 : 1) : 0;
 }
 
@@ -485,7 +617,7 @@ int launch_decay_fwd(const DecayArgs& a, hipStream_t stream) {
   auto pass = a.in_f32 ? launch_pass<true> : launch_pass<false>;
   if (j.seg != nullptr) {
     pass(p, 1, kStates, stream);
-    pass(p, 1, kScan, stream);
+    if (!p.join) pass(p, 1, kScan, stream);
   }
   pass(p, 1, kOutputs, stream);
   return (int)hipGetLastError();
@@ -513,7 +645,7 @@ int launch_decay_bwd(const DecayArgs& a, hipStream_t stream) {
     p.job[0] = js;
     p.job[1] = jd;
     pass(p, 2, kStates, stream);
-    pass(p, 2, kScan, stream);
+    if (!p.join) pass(p, 2, kScan, stream);
   }
   DecayJob jq = js, jk = jd;
   jq.q = dy, jq.k = v, jq.v = k, jq.out = a.dq, jq.d = a.dv, jq.dv = a.d, jq.seg_trans = jq.in_trans = 1;

@@ -27,23 +27,35 @@ template <>
 struct DecayOps<false> {
   typedef uint16_t elem;
   typedef u32x4 frag;
-  static constexpr int kPad = 8;         // elements behind a row of an LDS tile
+  // Rows of an LDS tile are W elements; the 16-byte unit c of row r lies at c ^ swizzle(r), under which no access here
+  // has more bank conflicts than its shape forces: 16-byte reads take the lanes of equal lane / 32 and equal parity of
+  // lane bits 2..4 in one pass over 64 banks, transposed ones 32 consecutive lanes.
+  template <int W>
+  static __device__ __forceinline__ int swizzle(int r) {
+    const int r2 = (r >> 2) & 1, r23 = ((r >> 2) ^ (r >> 3)) & 1;
+    if constexpr (W == 32) return r2 | r23 << 1;
+    if constexpr (W == 64) return r2 | (r & 2) | r23 << 2;
+    return r2 | (r & 3) << 1 | r23 << 3;
+  }
+  static constexpr int row_elems(int W) { return W; }
+  template <int W>
+  static __device__ __forceinline__ int at(int r, int c) { return r * W + ((c >> 3 ^ swizzle<W>(r)) << 3) + (c & 7); }
   static constexpr int kPair = 2;        // parts of a score or state entry in a bf16 product
   static constexpr int kFine = 3;        // parts of a weighted value in the state's update
   static __device__ __forceinline__ f32x4 mma(const frag& a, const frag& b, f32x4 c) { return mfma16x16x32(a, b, c); }
+  // Columns 8 c .. + 7 of row r; at(r, 8 c) + the elements of 16 whole rows more, or of another tile
   static __device__ __forceinline__ frag row(const elem* p) { return *reinterpret_cast<const u32x4*>(p); }
-  static __device__ __forceinline__ frag rows4(const elem* p0, const elem* p1) {
-    const u32x2 a = *reinterpret_cast<const u32x2*>(p0), b = *reinterpret_cast<const u32x2*>(p1);
-    return (u32x4){a[0], a[1], b[0], b[1]};
+  // Rows 8 g .. + 7 of one column for each lane of a 16-lane group: columns c0 + STEP j .. + 3 for lanes 4 j .. 4 j + 3.  Two
+  // transposed reads of four rows, in each of which lane i of the group addresses four columns of row i / 4.
+  template <int W, int STEP>
+  static __device__ __forceinline__ int col_at(int half, int c0, int lane) {
+    return at<W>(8 * (lane >> 4 & 3) + (lane >> 2 & 3) + 4 * half, c0 + STEP * (lane & 3));
   }
-  // Column c0 + l % 16 of rows row0 + 8 g .. + 7 of a row-major tile: two transposed reads of four rows,
-  // in each of which a 16-lane group's lane i addresses four columns of row i / 4.
-  static __device__ __forceinline__ frag col(const elem* tile, int ld, int row0, int c0, int lane) {
+  template <int W>
+  static __device__ __forceinline__ frag col(const elem* p0, const elem* p1) {
     typedef short v4s __attribute__((ext_vector_type(4)));
-    const int i = lane & 15, g = lane >> 4;
-    const elem* p = tile + (row0 + 8 * g + (i >> 2)) * ld + c0 + 4 * (i & 3);
-    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)p));
-    const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(p + 4 * ld)));
+    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)p0));
+    const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)p1));
     return (u32x4){a[0], a[1], b[0], b[1]};
   }
   static __device__ __forceinline__ f32x8 widen(const frag& a) {
@@ -75,7 +87,9 @@ template <>
 struct DecayOps<true> {
   typedef float elem;
   typedef f32x8 frag;
-  static constexpr int kPad = 4;
+  static constexpr int row_elems(int W) { return W + 4; }
+  template <int W>
+  static __device__ __forceinline__ int at(int r, int c) { return r * (W + 4) + c; }
   static constexpr int kPair = 1;
   static constexpr int kFine = 1;
   static __device__ __forceinline__ f32x4 mma(const frag& a, const frag& b, f32x4 c) {
@@ -83,16 +97,19 @@ struct DecayOps<true> {
     for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e], b.v[e], c, 0, 0, 0);
     return c;
   }
-  static __device__ __forceinline__ frag row(const elem* p) { return rows4(p, p + 4); }
-  static __device__ __forceinline__ frag rows4(const elem* p0, const elem* p1) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p0), b = *reinterpret_cast<const f32x4*>(p1);
+  static __device__ __forceinline__ frag row(const elem* p) {
+    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
     return {{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
   }
-  static __device__ __forceinline__ frag col(const elem* tile, int ld, int row0, int c0, int lane) {
-    const elem* p = tile + (row0 + 8 * (lane >> 4)) * ld + c0 + (lane & 15);
+  template <int W, int STEP>
+  static __device__ __forceinline__ int col_at(int half, int c0, int lane) {
+    return at<W>(8 * (lane >> 4 & 3) + 4 * half, c0 + STEP * (lane >> 2 & 3) + (lane & 3));
+  }
+  template <int W>
+  static __device__ __forceinline__ frag col(const elem* p0, const elem* p1) {
     frag r;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) r.v[e] = p[e * ld];
+    for (int e = 0; e < 4; ++e) r.v[e] = p0[e * (W + 4)], r.v[4 + e] = p1[e * (W + 4)];
     return r;
   }
   static __device__ __forceinline__ f32x8 widen(const frag& a) { return a; }
@@ -102,6 +119,14 @@ struct DecayOps<true> {
     p[0] = x;
   }
 };
+
+// A barrier for LDS alone: a work-group's global loads and stores stay in flight (__syncthreads() waits for them).
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 // A (B, H, N, w) operand: element (b, h, t, i) at p + b s[0] + h s[1] + t s[2] + i.
 struct DecayTensor {
