@@ -224,6 +224,31 @@ def test_strides_and_alignment(dtype):
     assert bool(((dk.double() - want).abs() <= 2.0 ** -7 * dkf.double().abs().sum(1, keepdim=True)).all())
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_expanded_tokens(dtype):
+    """One row for all tokens (stride 0), at a length that no chunk divides: rows behind it are no tokens."""
+    K = _K()
+    x = make(1, 3, 70, 64, 64, dtype, 8)
+    for n in "qkv":
+        one = {m: x[m].clone() for m in "qkv"}
+        one[n] = x[n][:, :, :1].expand(-1, -1, 70, -1)
+        y, st = K.decay_linear_attn(*(one[m] for m in "qkv"), x["g"], return_state=True)
+        one[n] = one[n].contiguous()
+        want, wst = K.decay_linear_attn(*(one[m] for m in "qkv"), x["g"], return_state=True)
+        assert torch.equal(y, want) and torch.equal(st, wst)
+
+
+def test_second_derivatives_are_refused():
+    K = _K()
+    x = make(1, 2, 20, 16, 16, F32, 3)
+    q = x["q"].requires_grad_()
+    y = K.decay_linear_attn(q, x["k"], x["v"], x["g"])
+    dq, = torch.autograd.grad(y, q, x["dy"], create_graph=True)
+    assert torch.equal(dq, torch.autograd.grad(K.decay_linear_attn(q, x["k"], x["v"], x["g"]), q, x["dy"])[0])
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dq.sum(), q)
+
+
 def test_types_through_fp32():
     K = _K()
     x = make(1, 2, 100, 16, 16, F32, 3)

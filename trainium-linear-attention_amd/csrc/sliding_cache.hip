@@ -51,6 +51,14 @@ __device__ __forceinline__ u32 rescale4(u32 w, float f) {
                  __builtin_amdgcn_cvt_f32_fp8((int)w, 2) * f, __builtin_amdgcn_cvt_f32_fp8((int)w, 3) * f);
 }
 
+// Bytes t .. t + 3 of a mask of valid places lo .. hi - 1.
+__device__ __forceinline__ u32 byte_mask(int t, int lo, int hi) {
+  u32 m = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) m |= t + j >= lo && t + j < hi ? 0xffu << (8 * j) : 0u;
+  return m;
+}
+
 struct CacheParams {
   DecayTensor k, v;
   uint8_t* kc;
@@ -63,46 +71,49 @@ struct CacheParams {
   int HK, N, d, dv, blocks, in_f32;
 };
 
-struct f8 {
-  float v[8];
-};
-
-// Elements col .. col + 7 of a row of w, zeros behind it.
-__device__ __forceinline__ f8 load8(const DecayTensor& x, size_t at, int col, int w, bool there, int f32) {
-  f8 r;
+// Elements col .. col + E - 1 of a row of w, zeros behind it.
+template <int E>
+__device__ __forceinline__ void load_row(const DecayTensor& x, size_t at, int col, int w, bool there, int f32, float (&r)[E]) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) r.v[j] = 0.f;
-  if (!there || col >= w) return r;
+  for (int j = 0; j < E; ++j) r[j] = 0.f;
+  if (!there || col >= w) return;
   if (f32) {
     const float* s = static_cast<const float*>(x.p) + at + col;
-    if (x.vec && col + 8 <= w) {
-      const f32x4 a = *reinterpret_cast<const f32x4*>(s), b = *reinterpret_cast<const f32x4*>(s + 4);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r.v[j] = a[j], r.v[4 + j] = b[j];
-    } else {
+    for (int i = 0; i < E; i += 4) {
+      if (x.vec && col + i < w) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(s + i);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (col + j < w) r.v[j] = s[j];
+        for (int j = 0; j < 4; ++j) r[i + j] = a[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col + i + j < w) r[i + j] = s[i + j];
+      }
     }
   } else {
     const uint16_t* s = static_cast<const uint16_t*>(x.p) + at + col;
-    if (x.vec) {
-      const u32x4 a = *reinterpret_cast<const u32x4*>(s);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r.v[2 * j] = bf16_lo_to_f32(a[j]), r.v[2 * j + 1] = bf16_hi_to_f32(a[j]);
-    } else {
+    for (int i = 0; i < E; i += 8) {
+      if (x.vec && col + i < w) {
+        const u32x4 a = *reinterpret_cast<const u32x4*>(s + i);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (col + j < w) r.v[j] = bf16_bits_to_f32(s[j]);
+        for (int j = 0; j < 4; ++j) r[i + 2 * j] = bf16_lo_to_f32(a[j]), r[i + 2 * j + 1] = bf16_hi_to_f32(a[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (col + i + j < w) r[i + j] = bf16_bits_to_f32(s[i + j]);
+      }
     }
   }
-  return r;
 }
 
-// One block of one (sequence, cached head): blockIdx.x the block among those the call touches.
+// One block of one (sequence, cached head): blockIdx.x the block among those the call touches.  A thread has E columns
+// of a token: 16-byte stores of codes (8 at the narrowest rows, so that every thread has some).  HBM-bound.
 template <int DP, int DVP>
 __global__ __launch_bounds__(256) void cache_append_kernel(const CacheParams p) {
-  constexpr int KI = CB * DP / 8 / 256, VI = CB * DVP / 8 / 256, VROW = CB + 4;
+  constexpr int KE = DP >= 64 ? 16 : 8, VE = DVP >= 64 ? 16 : 8, KI = CB * DP / KE / 256, VI = CB * DVP / VE / 256;
+  constexpr int KP = DP / KE, VP = DVP / VE, VROW = CB + 4;
   __shared__ u32 top[2][4];
   __shared__ __attribute__((aligned(16))) uint8_t vt[DVP * VROW];
   const int tid = threadIdx.x, bh = blockIdx.y, b = bh / p.HK, hk = bh - b * p.HK;
@@ -120,22 +131,26 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const CacheParams p) 
   uint8_t* kc = p.kc + rec * (CB * DP);
   uint8_t* vc = p.vc + rec * (CB * DVP);
 
-  f8 kx[KI], vx[VI];
+  float kx[KI][KE], vx[VI][VE];
   u32 km = 0, vm = 0;
 #pragma unroll
   for (int i = 0; i < KI; ++i) {
-    const int at = tid + 256 * i, row = at / (DP / 8), t = lb * CB + row - from;
-    kx[i] = load8(p.k, kb + (size_t)t * p.k.s[2], at % (DP / 8) * 8, p.d, row >= kept && row < stop, p.in_f32);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) km = max(km, finite_mag(kx[i].v[j]));
+    const int at = tid + 256 * i, row = at / KP, t = lb * CB + row - from;
+    load_row<KE>(p.k, kb + (long long)t * p.k.s[2], at % KP * KE, p.d, row >= kept && row < stop, p.in_f32, kx[i]);
   }
 #pragma unroll
   for (int i = 0; i < VI; ++i) {
-    const int at = tid + 256 * i, row = at / (DVP / 8), t = lb * CB + row - from;
-    vx[i] = load8(p.v, vb + (size_t)t * p.v.s[2], at % (DVP / 8) * 8, p.dv, row >= kept && row < stop, p.in_f32);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) vm = max(vm, finite_mag(vx[i].v[j]));
+    const int at = tid + 256 * i, row = at / VP, t = lb * CB + row - from;
+    load_row<VE>(p.v, vb + (long long)t * p.v.s[2], at % VP * VE, p.dv, row >= kept && row < stop, p.in_f32, vx[i]);
   }
+#pragma unroll
+  for (int i = 0; i < KI; ++i)
+#pragma unroll
+    for (int j = 0; j < KE; ++j) km = max(km, finite_mag(kx[i][j]));
+#pragma unroll
+  for (int i = 0; i < VI; ++i)
+#pragma unroll
+    for (int j = 0; j < VE; ++j) vm = max(vm, finite_mag(vx[i][j]));
   km = wave_max_u32(km);
   vm = wave_max_u32(vm);
   if ((tid & 63) == 0) {
@@ -154,39 +169,39 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const CacheParams p) 
   }
 #pragma unroll
   for (int i = 0; i < KI; ++i) {
-    const int at = tid + 256 * i, row = at / (DP / 8);
-    u32x2* dst = reinterpret_cast<u32x2*>(kc + 8 * at);
-    u32x2 w;
-    if (row < kept) {
-      w = *dst;
-      w = (u32x2){rescale4(w[0], old_k * ik), rescale4(w[1], old_k * ik)};
-    } else {
+    const int at = tid + 256 * i, row = at / KP;
+    u32* dst = reinterpret_cast<u32*>(kc + KE * at);
+    u32 w[KE / 4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) kx[i].v[j] *= ik;
-      w = (u32x2){encode4(kx[i].v[0], kx[i].v[1], kx[i].v[2], kx[i].v[3]), encode4(kx[i].v[4], kx[i].v[5], kx[i].v[6], kx[i].v[7])};
-    }
-    *dst = w;
+    for (int j = 0; j < KE / 4; ++j)
+      w[j] = row < kept ? rescale4(dst[j], old_k * ik)
+                        : encode4(kx[i][4 * j] * ik, kx[i][4 * j + 1] * ik, kx[i][4 * j + 2] * ik, kx[i][4 * j + 3] * ik);
+    if constexpr (KE == 16) *reinterpret_cast<u32x4*>(dst) = (u32x4){w[0], w[1], w[2], w[3]};
+    else *reinterpret_cast<u32x2*>(dst) = (u32x2){w[0], w[1]};
   }
 #pragma unroll
   for (int i = 0; i < VI; ++i) {
-    const int at = tid + 256 * i, row = at / (DVP / 8), col = at % (DVP / 8) * 8;
+    const int at = tid + 256 * i, row = at / VP, col = at % VP * VE;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) vx[i].v[j] *= iv;
-    const u32 w0 = encode4(vx[i].v[0], vx[i].v[1], vx[i].v[2], vx[i].v[3]), w1 = encode4(vx[i].v[4], vx[i].v[5], vx[i].v[6], vx[i].v[7]);
+    for (int j = 0; j < VE; j += 4) {
+      const u32 w = encode4(vx[i][j] * iv, vx[i][j + 1] * iv, vx[i][j + 2] * iv, vx[i][j + 3] * iv);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      vt[(col + j) * VROW + row] = (uint8_t)(w0 >> (8 * j));
-      vt[(col + 4 + j) * VROW + row] = (uint8_t)(w1 >> (8 * j));
+      for (int k = 0; k < 4; ++k) vt[(col + j + k) * VROW + row] = (uint8_t)(w >> (8 * k));
     }
   }
   __syncthreads();
-  for (int i = tid; i < DVP * CB / 4; i += 256) {
-    const int col = i / (CB / 4), t = i % (CB / 4) * 4;
-    u32* dst = reinterpret_cast<u32*>(vc + col * CB + t);
-    u32 w = *reinterpret_cast<const u32*>(vt + col * VROW + t);
+  for (int i = tid; i < DVP * CB / 16; i += 256) {
+    const int col = i / (CB / 16), t = i % (CB / 16) * 16;
+    u32x4* dst = reinterpret_cast<u32x4*>(vc + col * CB + t);
+    const u32* src = reinterpret_cast<const u32*>(vt + col * VROW + t);
+    u32x4 w = {src[0], src[1], src[2], src[3]};
     if (t < kept) {
-      const u32 o = rescale4(*dst, old_v * iv), m = kept - t >= 4 ? 0xffffffffu : (1u << (8 * (kept - t))) - 1;
-      w = (w & ~m) | (o & m);
+      const u32x4 old = *dst;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const u32 m = byte_mask(t + 4 * j, 0, kept);
+        w[j] = (w[j] & ~m) | (rescale4(old[j], old_v * iv) & m);
+      }
     }
     *dst = w;
   }
@@ -196,11 +211,13 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const CacheParams p) 
 
 struct StepParams {
   const void* q;
+  const void* k;     // the new tokens (B, HK, d), (B, HK, dv), contiguous; null: they are in the cache already
+  const void* v;
   void* out;
-  const uint8_t* kc;
-  const uint8_t* vc;
-  const float* ks;
-  const float* vs;
+  uint8_t* kc;
+  uint8_t* vc;
+  float* ks;
+  float* vs;
   const int* lengths;
   float* part;       // (B H, splits, DVP + 2): O, maximum, sum; or null: one split
   int H, HK, G, d, dv, blocks, window, splits;
@@ -218,12 +235,43 @@ __device__ __forceinline__ u32x4 codes_bf16(u32 a, u32 b) {
                  __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true))};
 }
 
-// Bytes t .. t + 3 of a mask of valid places lo .. hi - 1.
-__device__ __forceinline__ u32 byte_mask(int t, int lo, int hi) {
+__device__ __forceinline__ float load_one(const void* p, size_t i, int f32) {
+  return f32 ? static_cast<const float*>(p)[i] : bf16_bits_to_f32(static_cast<const uint16_t*>(p)[i]);
+}
+
+// One row of w elements (lane l: elements l, l + 64) as the codes at base + STEP times the element, by one wave, into place
+// `at` of a block of BYTES codes; its first place clears the block, and a larger scale than before moves the block's codes
+// to it (zeros stay zeros).
+template <int W, int STEP, int BYTES>
+__device__ __forceinline__ void put_token(const void* row, size_t first, int w, int f32, uint8_t* block, uint8_t* base, float* scale, int at, int lane) {
+  float x[(W + 63) / 64];
   u32 m = 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) m |= t + j >= lo && t + j < hi ? 0xffu << (8 * j) : 0u;
-  return m;
+  for (int i = 0; i < (W + 63) / 64; ++i) {
+    x[i] = lane + 64 * i < w ? load_one(row, first + lane + 64 * i, f32) : 0.f;
+    m = max(m, finite_mag(x[i]));
+  }
+  const float old = at ? *scale : 0.f, s = fmaxf(pow2f(scale_exp(wave_max_u32(m))), old), inv = inv_pow2(s);
+  if (at == 0 || s != old) {
+#pragma unroll
+    for (int i = 0; i < BYTES / 1024; ++i) {
+      u32x4* dst = reinterpret_cast<u32x4*>(block + 16 * (lane + 64 * i));
+      u32x4 y = {0u, 0u, 0u, 0u};
+      if (at) {
+        y = *dst;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = rescale4(y[j], old * inv);
+      }
+      *dst = y;
+    }
+    if (lane == 0) *scale = s;
+    // other lanes' bytes of these pieces are written next
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  }
+#pragma unroll
+  for (int i = 0; i < (W + 63) / 64; ++i)
+    if (lane + 64 * i < W) base[(size_t)STEP * (lane + 64 * i)] = (uint8_t)encode4(x[i] * inv, 0.f, 0.f, 0.f);
 }
 
 // Work-group: up to 16 query heads of one cached head of one sequence, one split of its blocks, which the four
@@ -259,6 +307,17 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(const StepParams p) {
       }
     }
     DecayOps<false>::parts<NQ>(y, qf[x]);
+  }
+
+  // the new token, by the wave that takes its block, which is that wave's last
+  if (p.k != nullptr && s1 == b0 + nb && s1 > s0 && w == ((s1 - 1 - s0) & 3)) {
+    const int bhk = b * p.HK + hk, at = last % CB;
+    const size_t rec = (size_t)bhk * p.blocks + last / CB % p.blocks;
+    uint8_t *kb = p.kc + rec * (CB * DP), *vb = p.vc + rec * (CB * DVP);
+    put_token<DP, 1, CB * DP>(p.k, (size_t)bhk * p.d, p.d, p.in_f32, kb, kb + at * DP, p.ks + rec, at, lane);
+    put_token<DVP, CB, CB * DVP>(p.v, (size_t)bhk * p.dv, p.dv, p.in_f32, vb, vb + at, p.vs + rec, at, lane);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
   }
 
   float m = -INFINITY, l = 0.f;
@@ -386,22 +445,39 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(const StepParams p) {
   }
 }
 
-// A head's splits, in order.
+// A head's splits, in order, eight in flight.
 template <int DVP>
 __global__ __launch_bounds__(DVP < 64 ? 64 : DVP) void cache_combine_kernel(const StepParams p) {
   const size_t head = blockIdx.x;
-  const int c = threadIdx.x;
+  const int c = min((int)threadIdx.x, DVP - 1);
   const float* src = p.part + head * p.splits * (DVP + 2);
-  float m = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, src[s * (DVP + 2) + DVP]);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float sum = 0.f, y = 0.f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float f = exp2_raw(src[s * (DVP + 2) + DVP] - ref);
-    sum = __builtin_fmaf(src[s * (DVP + 2) + DVP + 1], f, sum);
-    if (c < DVP) y = __builtin_fmaf(src[s * (DVP + 2) + c], f, y);
+  float m = -INFINITY, sum = 0.f, y = 0.f;
+  for (int s0 = 0; s0 < p.splits; s0 += 8) {
+    float ms[8], ls[8], os[8], mx = m;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float* part = src + min(s0 + i, p.splits - 1) * (DVP + 2);
+      ms[i] = part[DVP];
+      ls[i] = part[DVP + 1];
+      os[i] = part[c];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (s0 + i >= p.splits) ms[i] = -INFINITY;
+      mx = fmaxf(mx, ms[i]);
+    }
+    const float ref = mx == -INFINITY ? 0.f : mx, fade = exp2_raw(m - ref);
+    sum *= fade;
+    y *= fade;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float f = exp2_raw(ms[i] - ref);
+      sum = __builtin_fmaf(ls[i], f, sum);
+      y = __builtin_fmaf(os[i], f, y);
+    }
+    m = mx;
   }
-  if (c >= p.dv) return;
+  if ((int)threadIdx.x >= p.dv) return;
   y = p.lengths[head / p.H] > 0 ? y / sum : 0.f;
   if (p.out_f32) static_cast<float*>(p.out)[head * p.dv + c] = y;
   else static_cast<uint16_t*>(p.out)[head * p.dv + c] = f32_to_bf16_bits(y);
@@ -449,11 +525,14 @@ int attn_dims(const StepParams& p, int B, hipStream_t stream) {
 #undef LA_CALL
 }
 
+#ifndef LA_CACHE_WGS
+#define LA_CACHE_WGS 2
+#endif
 // Splits of a sequence's blocks: work-groups for about two a CU, four blocks each at least.
 int decode_splits(int B, int H, int HK, int blocks, int window) {
   const long long groups = (long long)B * HK * ((H / HK + 15) / 16);
   const long long most = window > 0 ? std::min<long long>(blocks, (window + 2 * CB - 2) / CB) : blocks;
-  const long long want = (2LL * device_cu_count() + groups - 1) / groups;
+  const long long want = ((long long)LA_CACHE_WGS * device_cu_count() + groups - 1) / groups;
   return (int)std::max(1LL, std::min(want, (most + 3) / 4));
 }
 
@@ -480,15 +559,20 @@ int launch_sliding_append(const SlidingCacheArgs& a, hipStream_t stream) {
 }
 
 int launch_sliding_decode(const SlidingCacheArgs& a, hipStream_t stream) {
-  const int rc = launch_sliding_append(a, stream);
-  if (rc != 0) return rc;
   StepParams p{};
   p.q = a.q;
   p.out = a.out;
-  p.kc = static_cast<const uint8_t*>(a.kc);
-  p.vc = static_cast<const uint8_t*>(a.vc);
+  p.kc = static_cast<uint8_t*>(a.kc);
+  p.vc = static_cast<uint8_t*>(a.vc);
   p.ks = a.ks;
   p.vs = a.vs;
+  if (a.H / a.HK <= 16) {      // one work-group reads the last block, and writes the token to it first
+    p.k = a.k;
+    p.v = a.v;
+  } else {
+    const int rc = launch_sliding_append(a, stream);
+    if (rc != 0) return rc;
+  }
   p.lengths = a.lengths;
   p.H = a.H;
   p.HK = a.HK;

@@ -137,6 +137,21 @@ def check(rc: int, what: str) -> None:
         raise BasedLAError(f"{what} failed: {status_string(rc)} (status {rc})")
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def launch(dev: int, name: str, *args) -> None:
+    """Calls an entry point for tensors on device ``dev``, which need not be the current one."""
+    fn = getattr(_lib if _lib is not None else lib(), name)
+    if _current_device() == dev:
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args)
+    if rc != 0:
+        check(rc, name)
+
+
 def hip_runtimes_loaded():
     """Paths of every libamdhip64 mapped into this process (one is expected)."""
     paths = set()

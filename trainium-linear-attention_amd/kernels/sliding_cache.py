@@ -16,8 +16,8 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .decay_attention import _operand, _strides
-from .pytorch_attention import _as_kernel_input, _compute_dtype
+from .decay_attention import _KERNEL_TYPES, _kernel_row, _operand, _same_device, _strides
+from .pytorch_attention import _compute_dtype
 
 __all__ = ["SlidingCache", "sliding_cache", "sliding_cache_append", "sliding_decode_step"]
 
@@ -65,29 +65,30 @@ def sliding_cache(b, heads, tokens, d, dv=None, device="cuda"):
                         torch.zeros(b, heads, blocks, device=device), torch.zeros(b, heads, blocks, device=device), d, dv)
 
 
-def _check_cache(cache: SlidingCache, like: torch.Tensor):
-    _lib.require_gpu(like, cache.k, cache.v, cache.k_scale, cache.v_scale)
-    dp, dvp = _padded(cache.d), _padded(cache.dv)
-    if cache.k.dim() != 5:
+def _check_cache(cache: SlidingCache, like: torch.Tensor, dev: int):
+    """The cache's (b, hk, blocks), its arrays checked against each other."""
+    k, v, ks, vs, d, dv = cache
+    _same_device(dev, like, k, v, ks, vs)
+    if k.dim() != 5:
         raise _lib.BasedLAError("cache.k must be (b, hk, blocks, 64, dp)")
-    b, hk, blocks = cache.k.shape[:3]
-    if (cache.k.dtype != _E4M3 or cache.v.dtype != _E4M3 or cache.k.shape[3:] != (CACHE_BLOCK, dp)
-            or cache.v.shape != (b, hk, blocks, dvp, CACHE_BLOCK)):
-        raise _lib.BasedLAError(f"cache.k and cache.v must be float8_e4m3fn {(b, hk, blocks, CACHE_BLOCK, dp)} and "
-                                f"{(b, hk, blocks, dvp, CACHE_BLOCK)}")
-    for s in (cache.k_scale, cache.v_scale):
-        if s.dtype != torch.float32 or s.shape != (b, hk, blocks):
-            raise _lib.BasedLAError(f"cache scales must be fp32 {(b, hk, blocks)}")
-    if not all(x.is_contiguous() for x in cache[:4]):
+    b, hk, blocks, at, dp = k.shape
+    if (k.dtype != _E4M3 or v.dtype != _E4M3 or at != CACHE_BLOCK or dp != _padded(d)
+            or v.shape != (b, hk, blocks, _padded(dv), CACHE_BLOCK)):
+        raise _lib.BasedLAError(f"cache.k and cache.v must be float8_e4m3fn {(b, hk, blocks, CACHE_BLOCK, _padded(d))} and "
+                                f"{(b, hk, blocks, _padded(dv), CACHE_BLOCK)}")
+    shape = (b, hk, blocks)
+    if ks.dtype != torch.float32 or vs.dtype != torch.float32 or ks.shape != shape or vs.shape != shape:
+        raise _lib.BasedLAError(f"cache scales must be fp32 {shape}")
+    if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise _lib.BasedLAError("the cache's arrays must be contiguous: they are updated in place")
-    return b, hk, blocks
+    return shape
 
 
-def _counts(x, like, b, name):
+def _counts(x, like, dev, b, name):
     if x is None:
         return None
-    _lib.require_gpu(like, x)
-    if x.dtype != torch.int32 or tuple(x.shape) != (b,):
+    _same_device(dev, like, x)
+    if x.dtype != torch.int32 or x.dim() != 1 or x.shape[0] != b:
         raise _lib.BasedLAError(f"{name} must be int32 of shape ({b},)")
     return x.contiguous()
 
@@ -99,21 +100,20 @@ def sliding_cache_append(cache, k, v, start=None, lengths=None):
     k: (b, hk, t, d); v: (b, hk, t, dv), any strides.  ``start``: int32 (b,), default zeros (tokens before it
     have been appended before); ``lengths``: int32 (b,), default t (a batch padded on the right).
     """
-    b, hk, blocks = _check_cache(cache, k)
-    _lib.require_gpu(k, v)
+    dev = k.get_device()
+    b, hk, blocks = _check_cache(cache, k, dev)
+    _same_device(dev, k, v)
     if k.dim() != 4 or v.dim() != 4 or k.shape[:2] != (b, hk) or v.shape[:3] != k.shape[:3] \
             or k.shape[3] != cache.d or v.shape[3] != cache.dv:
         raise _lib.BasedLAError(f"k, v must be ({b}, {hk}, t, {cache.d}) and ({b}, {hk}, t, {cache.dv})")
     if k.dtype != v.dtype:
         raise _lib.BasedLAError("k, v must share one dtype")
-    start, lengths = _counts(start, k, b, "start"), _counts(lengths, k, b, "lengths")
+    start, lengths = _counts(start, k, dev, b, "start"), _counts(lengths, k, dev, b, "lengths")
     cdt = _compute_dtype(k.dtype)
-    kc, vc = (_operand(x.detach(), cdt) for x in (k, v))
-    rc = _lib.lib().la_sliding_cache_append(
-        _lib.ptr(kc), _lib.ptr(vc), _lib.dtype_code(cdt), _lib.ptr(cache.k), _lib.ptr(cache.v), _lib.ptr(cache.k_scale),
-        _lib.ptr(cache.v_scale), _lib.ptr(start), _lib.ptr(lengths), b, hk, k.shape[2], cache.d, cache.dv, blocks,
-        _strides(kc), _strides(vc), _lib.stream_of(k))
-    _lib.check(rc, "la_sliding_cache_append")
+    kc, vc = _operand(k.detach(), cdt), _operand(v.detach(), cdt)
+    _lib.launch(dev, "la_sliding_cache_append", kc.data_ptr(), vc.data_ptr(), _lib.dtype_code(cdt), cache.k.data_ptr(),
+                cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), _lib.ptr(start), _lib.ptr(lengths),
+                b, hk, k.shape[2], cache.d, cache.dv, blocks, _strides(kc), _strides(vc), _lib.stream_of(k))
 
 
 def sliding_decode_step(q, k, v, cache, lengths, window_size=None, scale=None):
@@ -126,38 +126,41 @@ def sliding_decode_step(q, k, v, cache, lengths, window_size=None, scale=None):
     sequence of 0 takes no part (its output is zero, its cache stays).  ``window_size`` None: every position
     that the cache holds whole blocks of, all of a sequence that fits it.  ``scale`` defaults to 1/sqrt(d).
     """
-    b, hk, blocks = _check_cache(cache, q)
-    _lib.require_gpu(q, k, v, lengths)
+    dev = q.get_device()
+    b, hk, blocks = _check_cache(cache, q, dev)
+    d, dv = cache.d, cache.dv
+    _same_device(dev, q, k, v)
     squeeze = q.dim() == 4
     if squeeze:
         if k.dim() != 4 or v.dim() != 4 or not (q.shape[2] == k.shape[2] == v.shape[2] == 1):
             raise _lib.BasedLAError("decode takes one token per head: shape (b, h, 1, d)")
         q, k, v = q[:, :, 0], k[:, :, 0], v[:, :, 0]
-    if q.dim() != 3 or k.shape != (b, hk, cache.d) or v.shape != (b, hk, cache.dv) or q.shape[0] != b \
-            or q.shape[2] != cache.d or hk < 1 or q.shape[1] % hk:
-        raise _lib.BasedLAError(f"q must be ({b}, h, {cache.d}) with h a multiple of {hk}, k ({b}, {hk}, {cache.d}), "
-                                f"v ({b}, {hk}, {cache.dv})")
-    if not (q.dtype == k.dtype == v.dtype):
+    qs = q.shape
+    if len(qs) != 3 or k.shape != (b, hk, d) or v.shape != (b, hk, dv) or qs[0] != b or qs[2] != d or hk < 1 or qs[1] % hk:
+        raise _lib.BasedLAError(f"q must be ({b}, h, {d}) with h a multiple of {hk}, k ({b}, {hk}, {d}), v ({b}, {hk}, {dv})")
+    dt = q.dtype
+    if k.dtype != dt or v.dtype != dt:
         raise _lib.BasedLAError("q, k, v must share one dtype")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         raise _lib.BasedLAError("sliding_decode_step has no gradient: call it under torch.no_grad()")
-    lengths = _counts(lengths, q, b, "lengths")
+    lengths = _counts(lengths, q, dev, b, "lengths")
+    if lengths is None:
+        raise _lib.BasedLAError(f"lengths must be int32 of shape ({b},)")
     window = 0 if window_size is None else int(window_size)
     if window_size is not None and not 1 <= window <= CACHE_BLOCK * (blocks - 1) + 1:
         raise _lib.BasedLAError(f"window_size must be >= 1 and at most {CACHE_BLOCK * (blocks - 1) + 1} for this cache "
                                 f"(tokens - 63): a window of w tokens needs a cache of w + 63")
-    h = q.shape[1]
-    cdt = _compute_dtype(q.dtype)
-    kdt = q.dtype if q.dtype in (torch.float32, torch.bfloat16) else torch.float32
-    qc, kc, vc = (_as_kernel_input(x, cdt) for x in (q, k, v))
-    out = torch.empty((b, h, 1, cache.dv) if squeeze else (b, h, cache.dv), dtype=kdt, device=q.device)
-    L = _lib.lib()
-    ws_bytes = int(L.la_sliding_decode_workspace_bytes(b, h, hk, cache.d, cache.dv, blocks, window))
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-    rc = L.la_sliding_decode_step(
-        _lib.ptr(qc), _lib.ptr(kc), _lib.ptr(vc), _lib.dtype_code(cdt), _lib.ptr(out), _lib.dtype_code(kdt),
-        _lib.ptr(cache.k), _lib.ptr(cache.v), _lib.ptr(cache.k_scale), _lib.ptr(cache.v_scale), _lib.ptr(lengths), b, h, hk,
-        cache.d, cache.dv, blocks, window, 1.0 / math.sqrt(cache.d) if scale is None else float(scale), _lib.ptr(ws),
-        ws_bytes, _lib.stream_of(q))
-    _lib.check(rc, "la_sliding_decode_step")
-    return out if out.dtype == q.dtype else out.to(q.dtype)
+    h = qs[1]
+    cdt = _compute_dtype(dt)
+    kdt = dt if dt in _KERNEL_TYPES else torch.float32
+    qc, kc, vc = _kernel_row(q, cdt), _kernel_row(k, cdt), _kernel_row(v, cdt)
+    out = torch.empty((b, h, 1, dv) if squeeze else (b, h, dv), dtype=kdt, device=q.device)
+    ws_ptr, ws_bytes = 0, _lib.lib().la_sliding_decode_workspace_bytes(b, h, hk, d, dv, blocks, window)
+    if ws_bytes:
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+        ws_ptr = ws.data_ptr()
+    _lib.launch(dev, "la_sliding_decode_step", qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), _lib.dtype_code(cdt), out.data_ptr(),
+                _lib.dtype_code(kdt), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+                cache.v_scale.data_ptr(), lengths.data_ptr(), b, h, hk, d, dv, blocks, window,
+                1.0 / math.sqrt(d) if scale is None else float(scale), ws_ptr, ws_bytes, _lib.stream_of(q))
+    return out if kdt == dt else out.to(dt)
