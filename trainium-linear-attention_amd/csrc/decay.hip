@@ -114,9 +114,11 @@ struct RowLoader {
   int rb;               // bytes between tokens (VEC)
   const elem* p;        // the next chunk's first row in memory, as if it had 64
   long long row;        // elements between tokens
-  int w;
+  int w, move;          // move: tokens in memory from one chunk to the next
 
-  __device__ __forceinline__ void init(const DecayTensor& t, int b, int h, int width, int rev, int first, int len, int tid) {
+  // from the chunk at row `first` on, forwards (step 1) or backwards (step -1)
+  __device__ __forceinline__ void init(const DecayTensor& t, int b, int h, int width, int rev, int first, int step, int len, int tid) {
+    move = rev ? -C * step : C * step;
     row = t.s[2];
     w = width;
     rb = (int)(row * sizeof(elem));
@@ -144,7 +146,7 @@ struct RowLoader {
         x[i] = __builtin_bit_cast(u32x4, e);
       }
     }
-    p += rev ? -C * row : C * row;
+    p += move * row;
   }
   __device__ __forceinline__ void store(elem* tile, int tid) const {
 #pragma unroll
@@ -183,27 +185,31 @@ __global__ __launch_bounds__(4 * DVP) __attribute__((amdgpu_waves_per_eu(DP <= 6
   const int first = seg * p.seg_chunks * C, end = min(N, first + p.seg_chunks * C), stop = min(end, len);
   const int esz = p.out_f32 ? 4 : 2;
 
+  // A segment's own state is a sum in any order: it is taken from the segment's end, so that what this pass read last, the
+  // segments' beginnings, is what the outputs' pass reads first, while the memory-side cache still holds it.
+  const int begin = OUT || stop <= first ? first : first + (stop - 1 - first) / C * C, step = OUT ? C : -C;
   RowLoader<F32, DP, NT, VEC> ql, kl;
   RowLoader<F32, DVP, NT, VEC> vl;
-  if (OUT) ql.init(job.q, b, h, d, rev, first, len, tid);
-  kl.init(job.k, b, h, d, rev, first, len, tid);
-  vl.init(job.v, b, h, dv, rev, first, len, tid);
+  if (OUT) ql.init(job.q, b, h, d, rev, begin, OUT ? 1 : -1, len, tid);
+  kl.init(job.k, b, h, d, rev, begin, OUT ? 1 : -1, len, tid);
+  vl.init(job.v, b, h, dv, rev, begin, OUT ? 1 : -1, len, tid);
+  auto inside = [&](int r0) { return r0 >= first && r0 < stop; };
   // the rows of the chunk at r0 on their way
   auto load = [&](int r0) {
-    if (r0 >= stop) return;
+    if (!inside(r0)) return;
     const int n = min(C, stop - r0);
     if (OUT) ql.load(n, rev, tid);
     kl.load(n, rev, tid);
     vl.load(n, rev, tid);
   };
-  load(first);
+  load(begin);
   const float lg = log2_decay(p, h);
-  // .. and in the tiles, with the weights of its keys
+  // .. and in the tiles, with the weights of its keys: powers to the chunk's end, or the segment's
   auto put = [&](int r0, int buf) {
     if (OUT) ql.store(lds + QS, tid);
     kl.store(lds + buf * KT, tid);
     vl.store(lds + VS + buf * VT, tid);
-    if (tid < C) gv[buf][tid] = exp2_raw(lg * (float)max(min(C, stop - r0) - 1 - tid + rev, 0));
+    if (tid < C) gv[buf][tid] = exp2_raw(lg * (float)max((OUT ? min(C, stop - r0) : stop - r0) - 1 - tid + rev, 0));
   };
 
   // st[t][r] = S[state_row(t, g, r)][16 w + n16]
@@ -309,19 +315,19 @@ __global__ __launch_bounds__(4 * DVP) __attribute__((amdgpu_waves_per_eu(DP <= 6
   const Fade whole(lg, C);
 
   if (first < stop) {
-    put(first, 0);
-    load(first + C);
+    put(begin, 0);
+    load(begin + step);
   }
   int buf = 0;
-  for (int r0 = first; r0 < stop; r0 += C) {
+  for (int r0 = begin; inside(r0); r0 += step) {
     const int n = min(C, stop - r0);      // tokens of this chunk
     int w0 = w;
     asm volatile("" : "+s"(w0));      // addresses of score tiles are computed anew: their registers would cost a work-group a CU
     lds_barrier();      // tiles are whole, and the last chunk's P has been read
     const elem *kt_ = lds + buf * KT, *vt_ = lds + buf * VT;
-    if (!OUT && r0 + C < stop) {      // the other tiles have been read
-      put(r0 + C, buf ^ 1);
-      load(r0 + 2 * C);
+    if (!OUT && inside(r0 - C)) {      // the other tiles have been read
+      put(r0 - C, buf ^ 1);
+      load(r0 - 2 * C);
     }
     frag vf[2];
 #pragma unroll
@@ -379,15 +385,17 @@ __global__ __launch_bounds__(4 * DVP) __attribute__((amdgpu_waves_per_eu(DP <= 6
       __builtin_amdgcn_sched_barrier(0);
     }
     if (keep || r0 + C < stop) {      // S <- g^n S + K^T (weighted V)
-      const Fade fade = n == C ? whole : Fade(lg, n);
-      if (fade.slow) {
+      if (OUT) {
+        const Fade fade = n == C ? whole : Fade(lg, n);
+        if (fade.slow) {
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
+          for (int t = 0; t < DT; ++t)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) st[t][r] = __builtin_fmaf(st[t][r], fade.f, st[t][r]);
-      } else {
+            for (int r = 0; r < 4; ++r) st[t][r] = __builtin_fmaf(st[t][r], fade.f, st[t][r]);
+        } else {
 #pragma unroll
-        for (int t = 0; t < DT; ++t) st[t] *= fade.f;
+          for (int t = 0; t < DT; ++t) st[t] *= fade.f;
+        }
       }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
@@ -516,7 +524,7 @@ int pad_dim(int x) { return x <= 32 ? 32 : x <= 64 ? 64 : 128; }
 #define LA_DECAY_JOIN 131072
 #endif
 
-// Segments of a sequence: enough work-groups for the chip, of at least four chunks; two where the states of a head's
+// Segments of a sequence: enough work-groups for the chip, of at least four or six chunks; two where the states of a head's
 // segments are so few bytes that each segment adds up those before it, without a scan.
 struct Segments {
   int n, chunks;
@@ -525,7 +533,8 @@ struct Segments {
 Segments segments(long long BH, int N, int d, int dv) {
   const int chunks = (N + C - 1) / C, few = LA_DECAY_JOIN / (pad_dim(d) * pad_dim(dv) * (int)sizeof(float));
   const long long want = (long long)LA_DECAY_WGS * device_cu_count() / BH;
-  long long n = std::min(want, (long long)(chunks / 4));
+  const int least = pad_dim(d) * pad_dim(dv) > 8192 ? 6 : 4;      // a state's bytes are those of eight chunks' keys at 128 x 128
+  long long n = std::min(want, (long long)(chunks / least));
   if (n < few) n = std::min({want, (long long)(chunks / 2), (long long)few});
   n = std::max(1LL, n);
   Segments s{};

@@ -71,49 +71,42 @@ struct CacheParams {
   int HK, N, d, dv, blocks, in_f32;
 };
 
-// Elements col .. col + E - 1 of a row of w, zeros behind it.
-template <int E>
-__device__ __forceinline__ void load_row(const DecayTensor& x, size_t at, int col, int w, bool there, int f32, float (&r)[E]) {
+// Columns col .. col + E - 1 of row r of a block's new rows from .. to - 1 (x: row `from`), zeros in other rows and behind
+// a row of w.  VEC: through a buffer over these rows, so that no load waits for a branch.
+template <bool F32, bool VEC, int E>
+__device__ __forceinline__ void load_row(const void* x, long long stride, int r, int from, int to, int col, int w, float (&y)[E]) {
+  constexpr int Z = F32 ? 4 : 2;
+  if constexpr (VEC) {
+    const auto rs = make_rsrc(x, (u32)((to - from - 1) * (int)stride + w) * Z);
+    const int at = ((r - from) * (int)stride + col) * Z;
+    u32x4 a[E * Z / 16];
 #pragma unroll
-  for (int j = 0; j < E; ++j) r[j] = 0.f;
-  if (!there || col >= w) return;
-  if (f32) {
-    const float* s = static_cast<const float*>(x.p) + at + col;
+    for (int i = 0; i < E * Z / 16; ++i) a[i] = buf_load_b128(rs, col + i * 16 / Z < w ? at + 16 * i : kOffOutOfRange);
 #pragma unroll
-    for (int i = 0; i < E; i += 4) {
-      if (x.vec && col + i < w) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(s + i);
+    for (int i = 0; i < E * Z / 16; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) r[i + j] = a[j];
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (col + i + j < w) r[i + j] = s[i + j];
+      for (int j = 0; j < 4; ++j) {
+        const u32 z = a[i][j];
+        if constexpr (F32) y[4 * i + j] = __builtin_bit_cast(float, z);
+        else y[8 * i + 2 * j] = bf16_lo_to_f32(z), y[8 * i + 2 * j + 1] = bf16_hi_to_f32(z);
       }
-    }
   } else {
-    const uint16_t* s = static_cast<const uint16_t*>(x.p) + at + col;
+    const bool there = r >= from && r < to;
+    const long long at = (r - from) * stride + col;
 #pragma unroll
-    for (int i = 0; i < E; i += 8) {
-      if (x.vec && col + i < w) {
-        const u32x4 a = *reinterpret_cast<const u32x4*>(s + i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) r[i + 2 * j] = bf16_lo_to_f32(a[j]), r[i + 2 * j + 1] = bf16_hi_to_f32(a[j]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (col + i + j < w) r[i + j] = bf16_bits_to_f32(s[i + j]);
-      }
+    for (int j = 0; j < E; ++j) {
+      y[j] = 0.f;
+      if (there && col + j < w) y[j] = F32 ? static_cast<const float*>(x)[at + j] : bf16_bits_to_f32(static_cast<const uint16_t*>(x)[at + j]);
     }
   }
 }
 
 // One block of one (sequence, cached head): blockIdx.x the block among those the call touches.  A thread has E columns
 // of a token: 16-byte stores of codes (8 at the narrowest rows, so that every thread has some).  HBM-bound.
-template <int DP, int DVP>
+template <bool F32, int DP, int DVP, bool VEC>
 __global__ __launch_bounds__(256) void cache_append_kernel(const CacheParams p) {
   constexpr int KE = DP >= 64 ? 16 : 8, VE = DVP >= 64 ? 16 : 8, KI = CB * DP / KE / 256, VI = CB * DVP / VE / 256;
-  constexpr int KP = DP / KE, VP = DVP / VE, VROW = CB + 4;
+  constexpr int KP = DP / KE, VP = DVP / VE, VROW = CB + 4, Z = F32 ? 4 : 2;
   __shared__ u32 top[2][4];
   __shared__ __attribute__((aligned(16))) uint8_t vt[DVP * VROW];
   const int tid = threadIdx.x, bh = blockIdx.y, b = bh / p.HK, hk = bh - b * p.HK;
@@ -127,7 +120,9 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const CacheParams p) 
   if (lb + p.blocks <= (end - 1) / CB) return;                // taken over later in this call
   const int kept = max(from - lb * CB, 0), stop = min(end - lb * CB, CB);
   const size_t rec = (size_t)bh * p.blocks + lb % p.blocks;
-  const size_t kb = (size_t)(b * p.k.s[0] + hk * p.k.s[1]), vb = (size_t)(b * p.v.s[0] + hk * p.v.s[1]);
+  const long long t0 = lb * CB + kept - from;                 // the block's first new token
+  const char* kg = static_cast<const char*>(p.k.p) + (b * p.k.s[0] + hk * p.k.s[1] + t0 * p.k.s[2]) * Z;
+  const char* vg = static_cast<const char*>(p.v.p) + (b * p.v.s[0] + hk * p.v.s[1] + t0 * p.v.s[2]) * Z;
   uint8_t* kc = p.kc + rec * (CB * DP);
   uint8_t* vc = p.vc + rec * (CB * DVP);
 
@@ -135,13 +130,13 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const CacheParams p) 
   u32 km = 0, vm = 0;
 #pragma unroll
   for (int i = 0; i < KI; ++i) {
-    const int at = tid + 256 * i, row = at / KP, t = lb * CB + row - from;
-    load_row<KE>(p.k, kb + (long long)t * p.k.s[2], at % KP * KE, p.d, row >= kept && row < stop, p.in_f32, kx[i]);
+    const int at = tid + 256 * i;
+    load_row<F32, VEC, KE>(kg, p.k.s[2], at / KP, kept, stop, at % KP * KE, p.d, kx[i]);
   }
 #pragma unroll
   for (int i = 0; i < VI; ++i) {
-    const int at = tid + 256 * i, row = at / VP, t = lb * CB + row - from;
-    load_row<VE>(p.v, vb + (long long)t * p.v.s[2], at % VP * VE, p.dv, row >= kept && row < stop, p.in_f32, vx[i]);
+    const int at = tid + 256 * i;
+    load_row<F32, VEC, VE>(vg, p.v.s[2], at / VP, kept, stop, at % VP * VE, p.dv, vx[i]);
   }
 #pragma unroll
   for (int i = 0; i < KI; ++i)
@@ -220,9 +215,9 @@ struct StepParams {
   float* vs;
   const int* lengths;
   float* part;       // (B H, splits, DVP + 2): O, maximum, sum; or null: one split
-  int H, HK, G, d, dv, blocks, window, splits;
+  int H, HK, G, d, dv, blocks, window, splits, per;      // per: blocks of a split
   float scale;
-  int in_f32, out_f32;
+  int in_f32, out_f32, q_vec;      // q_vec: rows of q are whole 16-byte pieces (bf16)
 };
 
 typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf2;
@@ -289,24 +284,31 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(const StepParams p) {
   // positions p0 .. last, in blocks b0 .. b1 - 1; this split's of them
   int p0 = max(0, (last / CB + 1 - p.blocks) * CB);
   if (p.window > 0) p0 = max(p0, len - p.window);
-  const int b0 = p0 / CB, nb = len > 0 ? last / CB + 1 - b0 : 0, per = (nb + p.splits - 1) / p.splits;
+  const int b0 = p0 / CB, nb = len > 0 ? last / CB + 1 - b0 : 0, per = p.per;
   const int s0 = b0 + split * per, s1 = min(b0 + nb, s0 + per);
 
-  // Q^T: head n16, dims in the order of the key loads
+  // Q^T: head n16, dims in the order of the key loads; heads behind the last and dims behind d are zeros
+  const size_t qat = ((size_t)b * p.H + h0) * p.d;
+  constexpr int Z = F32 ? 4 : 2;
+  const auto qr = make_rsrc(static_cast<const char*>(p.q) + qat * Z, (u32)(nh * p.d * Z));
   u32x4 qf[KS][NQ];
 #pragma unroll
   for (int x = 0; x < KS; ++x) {
-    const int c = DP >= 64 ? 64 * (x / 2) + 16 * g + 8 * (x & 1) : 8 * g;
-    f32x8 y;
+    const int c = DP >= 64 ? 64 * (x / 2) + 16 * g + 8 * (x & 1) : 8 * g, at = (n16 * p.d + c) * Z;
+    if constexpr (F32) {
+      f32x8 y;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      y.v[j] = 0.f;
-      if (n16 < nh && c + j < p.d) {
-        const size_t at = ((size_t)b * p.H + h0 + n16) * p.d + c + j;
-        y.v[j] = p.in_f32 ? static_cast<const float*>(p.q)[at] : bf16_bits_to_f32(static_cast<const uint16_t*>(p.q)[at]);
-      }
+      for (int j = 0; j < 8; ++j)
+        y.v[j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(qr, c + j < p.d ? at + 4 * j : kOffOutOfRange, 0, 0));
+      DecayOps<false>::parts<NQ>(y, qf[x]);
+    } else if (p.q_vec) {
+      qf[x][0] = buf_load_b128(qr, c < p.d ? at : kOffOutOfRange);
+    } else {
+      uint16_t e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(qr, c + j < p.d ? at + 2 * j : kOffOutOfRange, 0, 0);
+      qf[x][0] = __builtin_bit_cast(u32x4, e);
     }
-    DecayOps<false>::parts<NQ>(y, qf[x]);
   }
 
   // the new token, by the wave that takes its block, which is that wave's last
@@ -485,8 +487,16 @@ __global__ __launch_bounds__(DVP < 64 ? 64 : DVP) void cache_combine_kernel(cons
 
 template <int DP, int DVP>
 int launch_append(const CacheParams& p, int BHK, hipStream_t stream) {
-  const int nb = (p.N + 2 * CB - 2) / CB;       // blocks that N tokens may touch
-  hipLaunchKernelGGL((cache_append_kernel<DP, DVP>), dim3((unsigned)nb, (unsigned)BHK), dim3(256), 0, stream, p);
+  const dim3 grid((unsigned)((p.N + 2 * CB - 2) / CB), (unsigned)BHK);      // blocks that N tokens may touch
+  const bool vec = p.k.vec && p.v.vec;
+  if (p.in_f32 && vec)
+    hipLaunchKernelGGL((cache_append_kernel<true, DP, DVP, true>), grid, dim3(256), 0, stream, p);
+  else if (p.in_f32)
+    hipLaunchKernelGGL((cache_append_kernel<true, DP, DVP, false>), grid, dim3(256), 0, stream, p);
+  else if (vec)
+    hipLaunchKernelGGL((cache_append_kernel<false, DP, DVP, true>), grid, dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL((cache_append_kernel<false, DP, DVP, false>), grid, dim3(256), 0, stream, p);
   return (int)hipGetLastError();
 }
 
@@ -526,14 +536,17 @@ int attn_dims(const StepParams& p, int B, hipStream_t stream) {
 }
 
 #ifndef LA_CACHE_WGS
-#define LA_CACHE_WGS 2
+#define LA_CACHE_WGS 3
 #endif
-// Splits of a sequence's blocks: work-groups for about two a CU, four blocks each at least.
-int decode_splits(int B, int H, int HK, int blocks, int window) {
+// Splits of a sequence's blocks: work-groups for about three a CU where the longest window is that long, of four blocks (one a
+// wave) at least.  A split has the same number of blocks in every sequence, so that short ones end in fewer work-groups and
+// the chip's dispatch evens out a batch of unlike lengths.
+int decode_splits(int B, int H, int HK, int blocks, int window, int* per) {
   const long long groups = (long long)B * HK * ((H / HK + 15) / 16);
   const long long most = window > 0 ? std::min<long long>(blocks, (window + 2 * CB - 2) / CB) : blocks;
-  const long long want = ((long long)LA_CACHE_WGS * device_cu_count() + groups - 1) / groups;
-  return (int)std::max(1LL, std::min(want, (most + 3) / 4));
+  const long long want = std::max(1LL, (long long)LA_CACHE_WGS * device_cu_count() / groups);
+  *per = (int)std::max(4LL, (most + want - 1) / want);
+  return (int)((most + *per - 1) / *per);
 }
 
 }  // namespace
@@ -541,7 +554,8 @@ int decode_splits(int B, int H, int HK, int blocks, int window) {
 int sliding_cache_dim(int d) { return d < 1 || d > 128 ? 0 : d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 
 size_t sliding_decode_workspace_bytes(int B, int H, int HK, int dv, int blocks, int window) {
-  const int s = decode_splits(B, H, HK, blocks, window);
+  int per;
+  const int s = decode_splits(B, H, HK, blocks, window, &per);
   return s > 1 ? (size_t)B * H * s * (sliding_cache_dim(dv) + 2) * sizeof(float) : 0;
 }
 
@@ -549,7 +563,8 @@ int launch_sliding_append(const SlidingCacheArgs& a, hipStream_t stream) {
   const int e = a.in_f32 ? 4 : 8;
   auto operand = [&](const void* ptr, const long long* s, int w) {
     DecayTensor x{ptr, {s[0], s[1], s[2]}, 0};
-    x.vec = (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && w % e == 0 && s[0] % e == 0 && s[1] % e == 0 && s[2] % e == 0;
+    x.vec = (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && w % e == 0 && s[0] % e == 0 && s[1] % e == 0 && s[2] % e == 0 &&
+            s[2] >= w && s[2] * (32 / e) <= (1 << 23);      // rows apart, 64 of them within a buffer's offsets
     return x;
   };
   const CacheParams p{operand(a.k, a.k_strides, a.d), operand(a.v, a.v_strides, a.dv), static_cast<uint8_t*>(a.kc),
@@ -581,11 +596,12 @@ int launch_sliding_decode(const SlidingCacheArgs& a, hipStream_t stream) {
   p.dv = a.dv;
   p.blocks = a.blocks;
   p.window = a.window;
-  p.splits = decode_splits(a.B, a.H, a.HK, a.blocks, a.window);
+  p.splits = decode_splits(a.B, a.H, a.HK, a.blocks, a.window, &p.per);
   p.part = p.splits > 1 ? static_cast<float*>(a.workspace) : nullptr;
   p.scale = a.scale;
   p.in_f32 = a.in_f32 ? 1 : 0;
   p.out_f32 = a.out_f32 ? 1 : 0;
+  p.q_vec = a.d % 8 == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0;
   return a.in_f32 ? attn_dims<true>(p, a.B, stream) : attn_dims<false>(p, a.B, stream);
 }
 
