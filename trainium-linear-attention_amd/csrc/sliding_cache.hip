@@ -327,11 +327,15 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(const StepParams p) {
 #pragma unroll
   for (int t = 0; t < MT; ++t) o[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
   const float c2 = p.scale * 1.44269504088896341f;
-  for (int blk = s0 + w; blk < s1; blk += 4) {
-    const size_t rec = ((size_t)b * p.HK + hk) * p.blocks + blk % p.blocks;
+  // A block's keys are loaded while the block before it takes its softmax and its values' product, and its values while its
+  // scores are computed: the registers are the same, and a wave has half a block on its way all the time.
+  u32x4 kx[4][KL], vx[MT];
+  float ks0 = 0.f, vs0 = 0.f;
+  auto record = [&](int blk) { return ((size_t)b * p.HK + hk) * p.blocks + blk % p.blocks; };
+  auto load_keys = [&](int blk) {
+    const size_t rec = record(blk);
     const uint8_t* kc = p.kc + rec * (CB * DP);
-    const uint8_t* vc = p.vc + rec * (CB * DVP);
-    u32x4 kx[4][KL], vx[MT];
+    ks0 = p.ks[rec] * c2;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const uint8_t* row = kc + ((n16 >> 2) * 16 + 4 * t + (n16 & 3)) * DP;
@@ -345,9 +349,20 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(const StepParams p) {
         }
       }
     }
+  };
+  auto load_values = [&](int blk) {
+    const size_t rec = record(blk);
+    const uint8_t* vc = p.vc + rec * (CB * DVP);
+    vs0 = p.vs[rec];
 #pragma unroll
     for (int t = 0; t < MT; ++t) vx[t] = *reinterpret_cast<const u32x4*>(vc + (16 * t + n16) * CB + 16 * g);
-    const float ksc = p.ks[rec] * c2, vsc = p.vs[rec];
+  };
+  if (s0 + w < s1) {
+    load_keys(s0 + w);
+    load_values(s0 + w);
+  }
+  for (int blk = s0 + w; blk < s1; blk += 4) {
+    const float ksc = ks0, vsc = vs0;
     f32x4 s[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -359,6 +374,7 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(const StepParams p) {
         for (int j = NQ - 1; j >= 0; --j) s[t] = mfma16x16x32(kf, qf[x][j], s[t]);
       }
     }
+    if (blk + 4 < s1) load_keys(blk + 4);
     const int lo = p0 - blk * CB, hi = len - blk * CB;     // valid places of the block
     const bool edge = lo > 0 || hi < CB;
     float mx = -INFINITY;
@@ -408,6 +424,7 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(const StepParams p) {
 #pragma unroll
         for (int j = NP - 1; j >= 0; --j) o[t] = mfma16x16x32(vf, pf[x][j], o[t]);
       }
+    if (blk + 4 < s1) load_values(blk + 4);
   }
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
@@ -535,16 +552,14 @@ int attn_dims(const StepParams& p, int B, hipStream_t stream) {
 #undef LA_CALL
 }
 
-#ifndef LA_CACHE_WGS
-#define LA_CACHE_WGS 3
-#endif
-// Splits of a sequence's blocks: work-groups for about three a CU where the longest window is that long, of four blocks (one a
-// wave) at least.  A split has the same number of blocks in every sequence, so that short ones end in fewer work-groups and
+// Splits of a sequence's blocks: as many work-groups as run at once, two a CU, where the longest window is that long (B8, 32 query
+// and 8 cached heads of 128 over up to 32768 tokens: 82 us, 96 with three and 85 with four), of four blocks (one a wave) at
+// least.  A split has the same number of blocks in every sequence, so that short ones end in fewer work-groups and
 // the chip's dispatch evens out a batch of unlike lengths.
 int decode_splits(int B, int H, int HK, int blocks, int window, int* per) {
   const long long groups = (long long)B * HK * ((H / HK + 15) / 16);
   const long long most = window > 0 ? std::min<long long>(blocks, (window + 2 * CB - 2) / CB) : blocks;
-  const long long want = std::max(1LL, (long long)LA_CACHE_WGS * device_cu_count() / groups);
+  const long long want = std::max(1LL, 2LL * device_cu_count() / groups);
   *per = (int)std::max(4LL, (most + want - 1) / want);
   return (int)((most + *per - 1) / *per);
 }
