@@ -189,6 +189,44 @@ def test_prompt_in_pieces_then_tokens():
         close(st[j:j + 1], wst, mst, F32, m + steps, "state")
 
 
+@pytest.mark.parametrize("g", [0.01, 0.5])
+def test_growth(g):
+    """Logarithms above 0: the same formula, while its numbers stay finite.  Powers of up to 2^92 have arguments that are
+    rounded once more, by 92 2^-24 of a power: 2^-17, in the state as in the outputs."""
+    x = make(1, 2, 128, 32, 32, F32, 2)
+    lg = torch.full((2,), g, device="cuda")
+    y, st = _K().decay_linear_attn(x["q"], x["k"], x["v"], lg, return_state=True)
+    want, wst = definition(*(x[n].double() for n in "qkv"), lg, 1 / math.sqrt(32))
+    mag, mst = definition(*(x[n].double().abs() for n in "qkv"), lg, 1 / math.sqrt(32))
+    assert float(((y - want).abs() / mag).max()) <= 2.0 ** -15 and float(((st - wst).abs() / mst).max()) <= 2.0 ** -15
+
+
+def test_backward_without_the_forward_states():
+    """la_decay_bwd computes the segments' states itself when the forward call's workspace is not given: same gradients,
+    to the bit."""
+    K = _K()
+    x = make(1, 3, 900, 64, 64, BF, 3, state=True, lengths=True)
+    leaves = [x[n].clone().requires_grad_() for n in ("q", "k", "v", "state")]
+    y = K.decay_linear_attn(*leaves[:3], x["g"], state_in=leaves[3], lengths=x["lengths"])
+    node = y.grad_fn
+    assert node.segments is not None
+    want = torch.autograd.grad(y, leaves, x["dy"], retain_graph=True)
+    node.segments = None
+    got = torch.autograd.grad(y, leaves, x["dy"])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_step_is_seen_by_autograd():
+    """A state that a differentiable call has saved and a step then changes: its gradient raises instead of being wrong."""
+    K = _K()
+    x = make(1, 2, 10, 16, 16, F32, 3, state=True)
+    q = x["q"].clone().requires_grad_()
+    y = K.decay_linear_attn(q, x["k"], x["v"], x["g"], state_in=x["state"])
+    K.decay_decode_step(x["q"][:, :, 0], x["k"][:, :, 0], x["v"][:, :, 0], x["g"], x["state"])
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, q, x["dy"])
+
+
 def test_no_decay_is_the_identity_map():
     K = _K()
     x = make(2, 3, 500, 32, 64, BF, 1)

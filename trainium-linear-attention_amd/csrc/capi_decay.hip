@@ -1,4 +1,5 @@
 // C-ABI entry points declared in include/based_la_decay.h: arguments are checked here, before any launch.
+#include <float.h>
 #include <math.h>
 
 #include "../../include/based_la.h"
@@ -17,8 +18,8 @@ bool overlap(const void* a, const void* b, size_t bytes) {
 int check_sizes(int B, int H, int N, int d, int dv, float scale) {
   if (B < 0 || H < 0 || N < 0 || d < 1 || dv < 1) return LA_ERR_BAD_SHAPE;
   if (d > 128 || dv > 128) return LA_ERR_UNSUPPORTED_DIM;
-  if ((long long)B * H > 0xffffffLL || (long long)N > 0x7fffff00LL) return LA_ERR_BAD_SHAPE;
-  if (!isfinite(scale) || !(scale > 0.f)) return LA_ERR_BAD_SCALAR;
+  if ((long long)B * H > 0xffffffLL || N > (1 << 30)) return LA_ERR_BAD_SHAPE;
+  if (!isfinite(scale) || !(scale >= FLT_MIN)) return LA_ERR_BAD_SCALAR;
   return LA_OK;
 }
 
@@ -39,7 +40,7 @@ extern "C" {
 
 size_t la_decay_workspace_bytes(int B, int H, int N, int d, int dv, int backward) {
   if (B < 1 || H < 1 || N < 1 || check_sizes(B, H, N, d, dv, 1.f) != LA_OK) return 0;
-  return la::decay_workspace_bytes((long long)B * H, N, d, dv, backward != 0);
+  return backward < 0 || backward > 1 ? 0 : la::decay_workspace_bytes((long long)B * H, N, d, dv, backward);
 }
 
 int la_decay_fwd(const void* q, const void* k, const void* v, int in_dtype, void* out, int out_dtype, int B, int H,
@@ -59,7 +60,7 @@ int la_decay_fwd(const void* q, const void* k, const void* v, int in_dtype, void
   if (!al(out, 16) || !al(log_decay, 4) || !al(lengths, 4) || !al(state_in, 16) || !al(state_out, 16))
     return LA_ERR_BAD_ALIGNMENT;
   if (overlap(state_in, state_out, (size_t)B * H * d * dv * 4)) return LA_ERR_OVERLAP;
-  const size_t need = la::decay_workspace_bytes((long long)B * H, N, d, dv, false);
+  const size_t need = la::decay_workspace_bytes((long long)B * H, N, d, dv, 0);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return LA_ERR_WORKSPACE;
   if (need > 0 && !al(workspace, 16)) return LA_ERR_BAD_ALIGNMENT;
   a.q = q;
@@ -86,7 +87,8 @@ int la_decay_bwd(const void* q, const void* k, const void* v, const void* dout, 
                  void* dv_out, int B, int H, int N, int d, int dv, const long long* q_strides,
                  const long long* k_strides, const long long* v_strides, const long long* dout_strides,
                  const float* log_decay, const int* lengths, float scale, const float* state_in,
-                 const float* dstate_out, float* dstate_in, void* workspace, size_t workspace_bytes, void* hip_stream) {
+                 const float* dstate_out, float* dstate_in, const void* fwd_workspace, void* workspace,
+                 size_t workspace_bytes, void* hip_stream) {
   int rc = check_sizes(B, H, N, d, dv, scale);
   if (rc != LA_OK) return rc;
   if (!dtype_ok(in_dtype)) return LA_ERR_BAD_DTYPE;
@@ -102,9 +104,11 @@ int la_decay_bwd(const void* q, const void* k, const void* v, const void* dout, 
       !al(dstate_out, 16) || !al(dstate_in, 16))
     return LA_ERR_BAD_ALIGNMENT;
   if (overlap(dstate_in, dstate_out, (size_t)B * H * d * dv * 4)) return LA_ERR_OVERLAP;
-  const size_t need = la::decay_workspace_bytes((long long)B * H, N, d, dv, true);
+  const size_t need = la::decay_workspace_bytes((long long)B * H, N, d, dv, fwd_workspace == nullptr);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return LA_ERR_WORKSPACE;
-  if (need > 0 && !al(workspace, 16)) return LA_ERR_BAD_ALIGNMENT;
+  if (need > 0 && (!al(workspace, 16) || !al(fwd_workspace, 16))) return LA_ERR_BAD_ALIGNMENT;
+  if (need > 0 && overlap(fwd_workspace, workspace, need)) return LA_ERR_OVERLAP;
+  a.fwd_states = static_cast<const float*>(fwd_workspace);
   a.q = q;
   a.k = k;
   a.v = v;

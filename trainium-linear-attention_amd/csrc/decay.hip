@@ -61,17 +61,18 @@ __device__ __forceinline__ int seq_len(const DecayParams& p, int b) {
 // log2 of the head's decay.  A decay of 0 has log -inf, for which 0 * log is no number: a large
 // negative one gives g^0 = 1 and g^n = 0.
 __device__ __forceinline__ float log2_decay(const DecayParams& p, int h) {
-  return fmaxf(p.log_decay[h], -1e30f) * 1.44269504088896341f;
+  const float x = p.log_decay[h];
+  return (x < -1e30f ? -1e30f : x) * 1.44269504088896341f;
 }
 
-// g^n for a state: x + x (g^n - 1) where g^n is above a half, which keeps slow decays exact over many
-// chunks (g^n itself rounds by 2^-24 each time), x g^n below, where g^n - 1 would cancel.
+// g^n for a state: x + x (g^n - 1) where g^n is between a half and two, which keeps slow decays exact over many
+// chunks (g^n itself rounds by 2^-24 each time), x g^n elsewhere (below, g^n - 1 would cancel).
 struct Fade {
   float f;
   bool slow;
   __device__ __forceinline__ Fade(float lg, int n) {
     const float e = lg * (float)n, x = e * 0.693147180559945309f;
-    slow = e > -1.f;
+    slow = fabsf(e) < 1.f;
     // e^x - 1 by its series, whose tenth term is below 2^-27 of the first for |x| <= ln 2
     float s = 1.f / 362880.f;
     const float c[8] = {1.f / 40320.f, 1.f / 5040.f, 1.f / 720.f, 1.f / 120.f, 1.f / 24.f, 1.f / 6.f, 0.5f, 1.f};
@@ -603,9 +604,9 @@ DecayParams common(const DecayArgs& a) {
 
 }  // namespace
 
-size_t decay_workspace_bytes(long long BH, int N, int d, int dv, bool backward) {
+size_t decay_workspace_bytes(long long BH, int N, int d, int dv, int backward) {
   const int n = segments(BH, N, d, dv).n;
-  return n > 1 ? (size_t)BH * n * pad_dim(d) * pad_dim(dv) * sizeof(float) * (backward ? 2 : 1) : 0;
+  return n > 1 ? (size_t)BH * n * pad_dim(d) * pad_dim(dv) * sizeof(float) * (backward + 1) : 0;
 }
 
 int launch_decay_fwd(const DecayArgs& a, hipStream_t stream) {
@@ -634,7 +635,8 @@ int launch_decay_fwd(const DecayArgs& a, hipStream_t stream) {
 
 // dq is the forward sum of (dy, v, k) from S^T; dk and dv are sums from the sequence's end, of (v, dy, q) from
 // dS^T and of (k, q, dy) from dS, where dS (not scaled by s) enters divided by s.  Two passes compute the
-// states of the segments, S of (k, v) and dS of (q, dy), which the three outputs' pass shares.
+// states of the segments, S of (k, v), if the forward pass's are not given, and dS of (q, dy), which the three outputs'
+// pass shares.
 int launch_decay_bwd(const DecayArgs& a, hipStream_t stream) {
   const DecayTensor q = operand(a.q, a.q_strides, a.d, a.in_f32), k = operand(a.k, a.k_strides, a.d, a.in_f32),
                     v = operand(a.v, a.v_strides, a.dv, a.in_f32), dy = operand(a.dout, a.dout_strides, a.dv, a.in_f32);
@@ -643,18 +645,19 @@ int launch_decay_bwd(const DecayArgs& a, hipStream_t stream) {
   auto pass = a.in_f32 ? launch_pass<true> : launch_pass<false>;
   float *s = nullptr, *ds = nullptr;
   if (p.nseg > 1) {
-    s = static_cast<float*>(a.workspace);
-    ds = s + (size_t)p.units * pad_dim(a.d) * pad_dim(a.dv);
+    ds = static_cast<float*>(a.workspace);
+    s = a.fwd_states != nullptr ? const_cast<float*>(a.fwd_states) : ds + (size_t)p.units * pad_dim(a.d) * pad_dim(a.dv);
   }
   DecayJob js{}, jd{};      // S, from the beginning, and dS, from the end
   js.k = k, js.v = v, js.seg = s, js.state_in = a.state_in, js.in_mul = js.out_mul = 1.f, js.d = a.d, js.dv = a.dv;
   jd.q = k, jd.k = q, jd.v = dy, jd.out = a.dv_out, jd.seg = ds, jd.state_in = a.dstate_out, jd.state_out = a.dstate_in;
   jd.in_mul = 1.f / a.scale, jd.out_mul = a.scale, jd.d = a.d, jd.dv = a.dv, jd.rev = 1, jd.fine = a.dstate_in != nullptr;
   if (p.nseg > 1) {
-    p.job[0] = js;
-    p.job[1] = jd;
-    pass(p, 2, kStates, stream);
-    if (!p.join) pass(p, 2, kScan, stream);
+    const int jobs = a.fwd_states != nullptr ? 1 : 2;      // the forward pass left S as it is needed
+    p.job[0] = jd;
+    p.job[1] = js;
+    pass(p, jobs, kStates, stream);
+    if (!p.join) pass(p, jobs, kScan, stream);
   }
   DecayJob jq = js, jk = jd;
   jq.q = dy, jq.k = v, jq.v = k, jq.out = a.dq, jq.d = a.dv, jq.dv = a.d, jq.seg_trans = jq.in_trans = 1;

@@ -102,6 +102,7 @@ struct DecayArgs {       // la_decay_fwd, la_decay_bwd
   float* state_out;
   const float* dstate_out;
   float* dstate_in;
+  const float* fwd_states;  // backward, optional: the workspace as the forward call left it
   const float* log_decay;   // (H)
   const int* lengths;       // optional, (B)
   long long q_strides[3], k_strides[3], v_strides[3], dout_strides[3];   // elements: batch, head, token
@@ -206,7 +207,7 @@ int device_cu_count();   // compute units of the current device (256 when the qu
 bool identity_shape(int d, int dv);
 size_t identity_workspace_bytes(int BH, int N, int d, int dv);
 int launch_identity(const IdentityArgs& a, hipStream_t stream);
-size_t decay_workspace_bytes(long long BH, int N, int d, int dv, bool backward);
+size_t decay_workspace_bytes(long long BH, int N, int d, int dv, int backward);   // state sets: backward + 1
 int launch_decay_fwd(const DecayArgs& a, hipStream_t stream);
 int launch_decay_bwd(const DecayArgs& a, hipStream_t stream);
 int launch_decay_step(const DecayStepArgs& a, hipStream_t stream);

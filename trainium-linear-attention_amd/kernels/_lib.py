@@ -85,7 +85,7 @@ _SIGNATURES = {
                               _c_void, _c_size, _c_void]),
     "la_decay_bwd": (_c_int, [_c_void, _c_void, _c_void, _c_void, _c_int, _c_void, _c_void, _c_void, _c_int, _c_int,
                               _c_int, _c_int, _c_int, _c_void, _c_void, _c_void, _c_void, _c_void, _c_void, _c_float,
-                              _c_void, _c_void, _c_void, _c_void, _c_size, _c_void]),
+                              _c_void, _c_void, _c_void, _c_void, _c_void, _c_size, _c_void]),
     "la_decay_step": (_c_int, [_c_void, _c_void, _c_void, _c_int, _c_void, _c_void, _c_void, _c_int, _c_int, _c_int,
                                _c_int, _c_int, _c_float, _c_void]),
     "la_sliding_cache_dim": (_c_int, [_c_int]),

@@ -90,7 +90,7 @@ def _forward(q, k, v, log_decay, lengths, scale, state_in, return_state, odt):
     _lib.launch(dev, "la_decay_fwd", qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), _lib.dtype_code(cdt), out.data_ptr(),
                 _lib.dtype_code(kdt), b, h, t, d, dv, _strides(qc), _strides(kc), _strides(vc), log_decay.data_ptr(),
                 _lib.ptr(lengths), scale, _lib.ptr(si), _lib.ptr(state), ws_ptr, ws_bytes, _lib.stream_of(q))
-    return (out if out.dtype == odt else out.to(odt)), state
+    return (out if out.dtype == odt else out.to(odt)), state, ws
 
 
 class _NoSecond(torch.autograd.Function):
@@ -110,7 +110,7 @@ class _DecayAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, log_decay, lengths, scale, state_in, return_state, odt):
-        y, state = _forward(q, k, v, log_decay, lengths, scale, state_in, return_state, odt)
+        y, state, ctx.segments = _forward(q, k, v, log_decay, lengths, scale, state_in, return_state, odt)
         ctx.save_for_backward(q, k, v, log_decay, lengths, state_in)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
@@ -144,11 +144,12 @@ def _backward(ctx, dy, dstate):
     dsi = torch.empty((b, h, d, dv), dtype=torch.float32, device=device) if want else None
     if t == 0 and want:
         dsi.zero_() if dso is None else dsi.copy_(dso)
-    ws, ws_ptr, ws_bytes = _workspace(dev, b, h, t, d, dv, 1, device)
+    seg = ctx.segments      # the forward pass's states of the segments, if it had any
+    ws, ws_ptr, ws_bytes = _workspace(dev, b, h, t, d, dv, 0 if seg is not None else 1, device)
     _lib.launch(dev, "la_decay_bwd", qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), dyc.data_ptr(), _lib.dtype_code(cdt),
                 dq.data_ptr(), dk.data_ptr(), dvo.data_ptr(), b, h, t, d, dv, _strides(qc), _strides(kc), _strides(vc),
                 _strides(dyc), log_decay.data_ptr(), _lib.ptr(lengths), ctx.scale, _lib.ptr(si), _lib.ptr(dso),
-                _lib.ptr(dsi), ws_ptr, ws_bytes, _lib.stream_of(q))
+                _lib.ptr(dsi), _lib.ptr(seg), ws_ptr, ws_bytes, _lib.stream_of(q))
     if cdt != q.dtype:
         dq, dk, dvo = dq.to(q.dtype), dk.to(q.dtype), dvo.to(q.dtype)
     return dq, dk, dvo, dsi
@@ -157,8 +158,8 @@ def _backward(ctx, dy, dstate):
 def decay_linear_attn(q, k, v, log_decay, scale=None, state_in=None, return_state=False, lengths=None, out_dtype=None):
     """Causal linear attention with a decay for each head, through ``la_decay_fwd`` / ``la_decay_bwd``.
 
-    q, k: (b, h, t, d); v: (b, h, t, dv), any strides; log_decay: fp32 (h,), <= 0 (-inf: each token sees
-    itself only).  ``scale`` defaults to 1/sqrt(d).  ``state_in``: fp32 (b, h, d, dv), an earlier call's
+    q, k: (b, h, t, d); v: (b, h, t, dv), any strides; log_decay: fp32 (h,), in general <= 0 (-inf: each token
+    sees itself only).  ``scale`` defaults to 1/sqrt(d).  ``state_in``: fp32 (b, h, d, dv), an earlier call's
     state that these tokens follow; ``return_state`` also returns the state after the last token, in the
     same layout, which ``decay_decode_step`` goes on from.  ``lengths``: int32 (b,), the tokens of each
     sequence of a batch padded on the right; rows behind them are not read, their outputs and gradients
@@ -185,7 +186,7 @@ def decay_linear_attn(q, k, v, log_decay, scale=None, state_in=None, return_stat
                                     or (state_in is not None and state_in.requires_grad)):
         y, state = _DecayAttention.apply(q, k, v, log_decay, lengths, scale, state_in, return_state, odt)
     else:
-        y, state = _forward(q, k, v, log_decay, lengths, scale, state_in, return_state, odt)
+        y, state, _ = _forward(q, k, v, log_decay, lengths, scale, state_in, return_state, odt)
     return (y, state) if return_state else y
 
 
@@ -228,4 +229,6 @@ def decay_decode_step(q, k, v, log_decay, state, scale=None):
     _lib.launch(dev, "la_decay_step", qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), _lib.dtype_code(cdt), log_decay.data_ptr(),
                 state.data_ptr(), out.data_ptr(), _lib.dtype_code(kdt), b, h, d, dv,
                 1.0 / math.sqrt(d) if scale is None else float(scale), _lib.stream_of(q))
+    if not state.is_inference():      # autograd has not seen the update in place
+        torch.autograd.graph.increment_version(state)
     return out if kdt == dt else out.to(dt)
