@@ -18,6 +18,13 @@
 // far from 64 bits as their own rounding.  Weighted values enter the update as two as well, or as three (24 bits)
 // where the state is an output, which is fp32 and has fp32's accuracy.  fp32 inputs run on fp32 matrix
 // instructions throughout.
+//
+// What bounds it, measured on the device.  d = dv = 64 in bf16 is bound by memory: B1 H16 N65536 takes 185 us, of which the
+// segments' pass 68 (reads 268 MB: 3.9 TB/s), the scan 9, the outputs' pass 106 (536 MB read and written: 5.1 TB/s).  Two
+// chunks on their way instead of one left both passes as they were.  d = dv = 128 is bound by a chunk's chain of
+// LDS reads and matrix products, with two work-groups a CU: B4 H8 N3001 takes 61 us (17 + 8 + 35).  Small calls are two or
+// three launches' latencies: B1 H4 N1024 in fp32 18 us.  The gradients of B2 H16 N8192 at d = dv = 64 take 106 us with
+// the states that the forward pass left.
 #include <math.h>
 
 #include <algorithm>
@@ -518,23 +525,23 @@ __global__ __launch_bounds__(kScanThreads) void decay_scan_kernel(const DecayPar
 
 int pad_dim(int x) { return x <= 32 ? 32 : x <= 64 ? 64 : 128; }
 
-#ifndef LA_DECAY_WGS
-#define LA_DECAY_WGS 3      // work-groups a CU that sequences are cut for
-#endif
-#ifndef LA_DECAY_JOIN
-#define LA_DECAY_JOIN 131072
-#endif
+// Work-groups a CU that sequences are cut for: as many as run at once at d = dv = 64 (2 to 8 measure alike but for what is
+// left over in the last round).
+constexpr int kWgsPerCu = 3;
+// Bytes of a head's segments' states up to which each segment adds up those before it, without a scan: B1 H4 N1024 in fp32 takes
+// 18 us so, 28 with the scan; at B2 H16 N2048, at the limit, the two are equal.
+constexpr int kJoinBytes = 1 << 17;
 
-// Segments of a sequence: enough work-groups for the chip, of at least four or six chunks; two where the states of a head's
-// segments are so few bytes that each segment adds up those before it, without a scan.
+// Segments of a sequence: enough work-groups for the chip, of at least four chunks, six where a state has more bytes than eight
+// chunks' keys (B4 H8 N3001 at 128 x 128: 61 us, 66 with four and 75 with eight); of two where nothing is scanned.
 struct Segments {
   int n, chunks;
   bool join;
 };
 Segments segments(long long BH, int N, int d, int dv) {
-  const int chunks = (N + C - 1) / C, few = LA_DECAY_JOIN / (pad_dim(d) * pad_dim(dv) * (int)sizeof(float));
-  const long long want = (long long)LA_DECAY_WGS * device_cu_count() / BH;
-  const int least = pad_dim(d) * pad_dim(dv) > 8192 ? 6 : 4;      // a state's bytes are those of eight chunks' keys at 128 x 128
+  const int chunks = (N + C - 1) / C, few = kJoinBytes / (pad_dim(d) * pad_dim(dv) * (int)sizeof(float));
+  const long long want = (long long)kWgsPerCu * device_cu_count() / BH;
+  const int least = pad_dim(d) * pad_dim(dv) > 8192 ? 6 : 4;
   long long n = std::min(want, (long long)(chunks / least));
   if (n < few) n = std::min({want, (long long)(chunks / 2), (long long)few});
   n = std::max(1LL, n);
