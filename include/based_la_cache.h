@@ -13,9 +13,11 @@
  * A block's scale is the smallest power of two, 2^-100 at the least, that brings its largest finite magnitude to
  * 448 or below; codes are rounded to nearest even, and infinities become NaN.  Where later tokens of a block
  * raise its scale, its earlier codes are rounded again under the new one.  Places behind a sequence's last
- * token are not read; an append writes zeros to those of its last block.  A token at the first place of a block takes the block over: the one of `blocks` blocks ago is gone.
+ * token are not read; an append writes zeros to those of its last block.  A token at the first place of a
+ * block takes the block over: the one of `blocks` blocks ago is gone.
  *
- * Limits: 1 <= d, dv <= 128 (LA_ERR_UNSUPPORTED_DIM), 1 <= blocks <= 2^24.
+ * Limits: 1 <= d, dv <= 128 (LA_ERR_UNSUPPORTED_DIM), 1 <= blocks <= 2^24, B HK <= 65535, N <= 2^29; of a step H <= 65535,
+ * B H < 2^24.
  */
 #ifndef BASED_LA_CACHE_H
 #define BASED_LA_CACHE_H

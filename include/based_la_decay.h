@@ -12,7 +12,8 @@
  * lengths: int32 (B) in device memory or NULL (L = N everywhere); values are taken between 0 and N.
  * Rows behind a sequence are not read, and their outputs and gradients are written as zeros.
  * A value that is not finite reaches, besides later outputs, those of its own 64 tokens (64 t .. 64 t + 63).
- * Limits: 1 <= d, dv <= 128 (LA_ERR_UNSUPPORTED_DIM), N <= 2^30, scale positive, finite and not subnormal.
+ * Limits: 1 <= d, dv <= 128 (LA_ERR_UNSUPPORTED_DIM), B H <= 2^21, N <= 2^30, scale positive, finite and not
+ * subnormal.  With B, H or N of 0 nothing is launched and nothing written.
  */
 #ifndef BASED_LA_DECAY_H
 #define BASED_LA_DECAY_H

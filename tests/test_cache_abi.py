@@ -40,13 +40,13 @@ BOTH = [(dict(k=None), -1), (dict(v=None), -1), (dict(kc=None), -1), (dict(vs=No
         (dict(B=70000), -2)]
 
 
-@pytest.mark.parametrize("kw,code", BOTH + [(dict(N=-1), -2), (dict(start=ODD), -8), (dict(kst=S3(0, -1, 0)), -2)])
+@pytest.mark.parametrize("kw,code", BOTH + [(dict(N=-1), -2), (dict(N=(1 << 29) + 1), -2), (dict(start=ODD), -8), (dict(kst=S3(0, -1, 0)), -2)])
 def test_append_refusals(kw, code):
     assert _lib().la_sliding_cache_append(*{**APPEND, **kw}.values(), None) == code
 
 
 @pytest.mark.parametrize("kw,code", BOTH + [(dict(q=None), -1), (dict(out=None), -1), (dict(lens=None), -1), (dict(H=5), -2),
-                                            (dict(HK=0), -2), (dict(window=-1), -2), (dict(window=194), -2), (dict(odt=7), -3),
+                                            (dict(HK=0), -2), (dict(window=-1), -2), (dict(window=194), -2), (dict(B=300, H=60000), -2), (dict(odt=7), -3),
                                             (dict(scale=0.0), -4), (dict(scale=float("nan")), -4),
                                             (dict(blocks=4096), -6), (dict(blocks=4096, ws=ODD, wsb=1 << 40), -8)])
 def test_step_refusals(kw, code):

@@ -61,7 +61,7 @@ FAR = ctypes.c_void_p(1 << 20)
 
 COMMON = [(dict(q=None), -1), (dict(k=None), -1), (dict(v=None), -1), (dict(g=None), -1), (dict(B=-1), -2), (dict(d=0), -2),
           (dict(dt=3), -3), (dict(scale=0.0), -4), (dict(scale=1e-40), -4), (dict(scale=float("inf")), -4), (dict(d=129), -5), (dict(dv=129), -5),
-          (dict(q=ctypes.c_void_p(65)), -8)]
+          (dict(q=ctypes.c_void_p(65)), -8), (dict(B=1 << 16, H=33), -2)]
 SEQ = COMMON + [(dict(N=-1), -2), (dict(N=(1 << 30) + 1), -2), (dict(qs=S3(0, 0, -1)), -2), (dict(si=ODD), -8), (dict(lens=ODD), -8),
                 (dict(N=100000), -6), (dict(N=100000, ws=ODD, wsb=1 << 40), -8)]
 

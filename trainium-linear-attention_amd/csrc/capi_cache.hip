@@ -13,8 +13,8 @@ bool dtype_ok(int t) { return t == LA_F32 || t == LA_BF16; }
 int check_sizes(int B, int HK, int N, int d, int dv, int blocks) {
   if (B < 0 || HK < 0 || N < 0 || d < 1 || dv < 1 || blocks < 1 || blocks > (1 << 24)) return LA_ERR_BAD_SHAPE;
   if (d > 128 || dv > 128) return LA_ERR_UNSUPPORTED_DIM;
-  // work-group indices of the launches
-  if (B > 0xffff || (long long)B * HK > 0xffff || N > 0x7fffff00) return LA_ERR_BAD_SHAPE;
+  // work-group indices and threads of the launches
+  if (B > 0xffff || (long long)B * HK > 0xffff || N > (1 << 29)) return LA_ERR_BAD_SHAPE;
   return LA_OK;
 }
 

@@ -18,7 +18,8 @@ bool overlap(const void* a, const void* b, size_t bytes) {
 int check_sizes(int B, int H, int N, int d, int dv, float scale) {
   if (B < 0 || H < 0 || N < 0 || d < 1 || dv < 1) return LA_ERR_BAD_SHAPE;
   if (d > 128 || dv > 128) return LA_ERR_UNSUPPORTED_DIM;
-  if ((long long)B * H > 0xffffffLL || N > (1 << 30)) return LA_ERR_BAD_SHAPE;
+  // three sums of 512 threads a head are one launch, of fewer than 2^32 threads
+  if ((long long)B * H > (1 << 21) || N > (1 << 30)) return LA_ERR_BAD_SHAPE;
   if (!isfinite(scale) || !(scale >= FLT_MIN)) return LA_ERR_BAD_SCALAR;
   return LA_OK;
 }
