@@ -388,3 +388,29 @@ def test_other_stream():
         y = K.decay_linear_attn(x["q"], x["k"], x["v"], x["g"])
     s.synchronize()
     assert torch.equal(y, want)
+
+
+def test_offsets_beyond_32_bits():
+    """One sequence of more than 2^31 elements: with g = e^-0.5 rows near an end see nothing of the other end (e^-128),
+    so that both ends are the definition's on 512 rows; outputs and gradients of the rows that lie in their inner half."""
+    N, d, cut = (1 << 24) + 77, 128, 512
+    g = torch.Generator(device="cuda").manual_seed(11)
+    q, k, v, dy = (torch.randn(1, 1, N, d, generator=g, device="cuda", dtype=BF) for _ in range(4))
+    lg = torch.tensor([-0.5], device="cuda")
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    y, st = _K().decay_linear_attn(*leaves, lg, return_state=True)
+    grads = [x.detach() for x in torch.autograd.grad(y, leaves, dy)]
+    y, st = y.detach(), st.detach()
+    for rows, half in ((slice(N - cut, N), slice(cut // 2, cut)), (slice(0, cut), slice(0, cut // 2))):
+        def formula(f):
+            w = [f(x.detach()[:, :, rows].double()).requires_grad_() for x in leaves]
+            yy, ss = definition(*w, lg, 1 / math.sqrt(d))
+            return [yy.detach(), ss.detach()] + list(torch.autograd.grad(yy, w, f(dy[:, :, rows].double())))
+        want, mag = formula(lambda t: t.clone()), formula(torch.abs)
+        at_end = rows.stop == N
+        names = ["y", "dq"] if at_end else ["y", "dq", "dk", "dv"]      # dk and dv look ahead
+        for n, a, w, m in zip(["y", "dq", "dk", "dv"], [y] + grads, want[:1] + want[2:], mag[:1] + mag[2:]):
+            if n in names:
+                close(a[:, :, rows][:, :, half], w[:, :, half], m[:, :, half], BF, d, n)
+        if at_end:
+            close(st, want[1], mag[1], F32, cut, "state")

@@ -331,3 +331,25 @@ def test_empty_batches():
     q = torch.randn(2, 2, 16, device="cuda")
     y = K.sliding_decode_step(q, q, q, cache, ints(0, -5))
     assert not y.any() and not cache.k.float().any() and not cache.k_scale.any()
+
+
+def test_offsets_beyond_32_bits():
+    """Positions around 2^25, where the codes lie 2^32 bytes from the first ones: the last blocks are the model's, the step
+    the definition's on them."""
+    K = _K()
+    lo, n, d, w = (1 << 19) - 2, 329, 128, 190      # from block lo on: 328 tokens, then one
+    g = torch.Generator(device="cuda").manual_seed(4)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").to(BF)  # noqa: E731
+    cache, model = K.sliding_cache(1, 1, 64 * (lo + 6), d), Model(1, 1, 6, d, d)
+    k, v = r(1, 1, n - 1, d), r(1, 1, n - 1, d)
+    K.sliding_cache_append(cache, k, v, start=ints(64 * lo))
+    model.append(k, v, [0], [n - 1])
+    q, k, v = r(1, 2, d), r(1, 1, d), r(1, 1, d)
+    y = K.sliding_decode_step(q, k, v, cache, ints(64 * lo + n), window_size=w)
+    model.append(k.unsqueeze(2), v.unsqueeze(2), [n - 1], [1])
+    tail = K.SlidingCache(*(x[:, :, lo:].contiguous() for x in cache[:4]), d, d)
+    assert not cache.k_scale[:, :, :lo].any() and not cache.v_scale[:, :, :lo].any()
+    del cache
+    model.check(tail)
+    want, A, S = attention(q, tail, (n,), w, 1 / math.sqrt(d))
+    close(y, want, A, S, BF, d, w)
