@@ -34,7 +34,8 @@ size_t la_decay_workspace_bytes(int B, int H, int N, int d, int dv, int backward
  * not overlap state_in (LA_ERR_OVERLAP).  Element (b, h, t, i) of an operand x lies at
  * x + b x_strides[0] + h x_strides[1] + t x_strides[2] + i (in elements, >= 0, NULL: contiguous); out is
  * contiguous and 16-byte aligned, and so are states and workspace.  Operands whose start and strides are
- * multiples of 16 bytes and whose rows are whole 16-byte pieces are read 16 bytes at a time, others by element.
+ * multiples of 16 bytes and whose rows are whole 16-byte pieces are read 16 bytes at a time, those of which this
+ * holds with 4 bytes by 4-byte words, others by element.
  */
 int la_decay_fwd(const void* q, const void* k, const void* v, int in_dtype, void* out, int out_dtype, int B, int H,
                  int N, int d, int dv, const long long* q_strides, const long long* k_strides,

@@ -414,3 +414,28 @@ def test_offsets_beyond_32_bits():
                 close(a[:, :, rows][:, :, half], w[:, :, half], m[:, :, half], BF, d, n)
         if at_end:
             close(st, want[1], mag[1], F32, cut, "state")
+
+
+@pytest.mark.parametrize("dtype,d,dv", [(BF, 100, 60), (BF, 6, 34), (BF, 62, 128), (F32, 63, 5), (F32, 101, 127), (BF, 33, 64)])
+def test_rows_of_words_and_of_elements(dtype, d, dv):
+    """Widths that are no whole 16-byte pieces, and a start in the middle of one: with zeros behind each row up to whole
+    pieces the terms are the same, and so are the bits of outputs, states and gradients."""
+    K, P = _K(), torch.nn.functional.pad
+    B, H, N = 2, 3, 333
+    x = make(B, H, N, d, dv, dtype, d, lengths=True, state=True)
+    pd, pv = -d % 8, -dv % 8
+    wide = {n: P(x[n], (0, pd if n in "qk" else pv)) for n in ("q", "k", "v", "dy")}
+    wide.update({n: P(x[n], (0, pv, 0, pd)) for n in ("state", "dstate")})
+
+    def call(t):
+        leaves = [t[n].detach().requires_grad_() for n in ("q", "k", "v", "state")]
+        y, st = K.decay_linear_attn(*leaves[:3], x["g"], scale=0.3, state_in=leaves[3], return_state=True, lengths=x["lengths"])
+        return [y, st] + list(torch.autograd.grad([y, st], leaves, [t["dy"], t["dstate"]]))
+
+    want = call(wide)
+    shifted = dict(x)      # rows of two elements more, from the second on
+    for n in ("q", "k", "v", "dy"):
+        shifted[n] = P(x[n], (2, 0))[..., 2:]
+    for t in (x, shifted):
+        for n, a, w in zip(("y", "state", "dq", "dk", "dv", "dstate"), call(t), want):
+            assert torch.equal(a.detach(), w.detach()[tuple(slice(0, s) for s in a.shape)]), n

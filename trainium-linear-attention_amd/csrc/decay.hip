@@ -91,6 +91,9 @@ struct Fade {
   __device__ __forceinline__ float operator()(float x) const { return __builtin_fmaf(x, f, slow ? x : 0.f); }
 };
 
+// How rows are read, by what they and their strides are made of (DecayTensor::vec).
+enum Rows { kElements, kWords, kPieces };
+
 // Where entry (kd, vd) of the head's state lies in state_in.
 __device__ __forceinline__ size_t state_at(int d, int dv, size_t bh, int kd, int vd, int trans) {
   return trans ? (bh * dv + vd) * d + kd : (bh * d + kd) * dv + vd;
@@ -110,17 +113,19 @@ __device__ __forceinline__ int unit_of(const DecayParams& p, int& job) {
 }
 
 // Chunks of a (b, h)'s rows on their way to an LDS tile of W columns, in registers, one chunk of 64 rows after
-// another: row r of the sequence is token r, or token len - 1 - r (rev).  VEC: rows are whole 16-byte pieces, read through
-// a buffer over the chunk's rows, so that rows behind the sequence and columns behind the row read as zeros without a branch.
-template <bool F32, int W, int NT, bool VEC>
+// another: row r of the sequence is token r, or token len - 1 - r (rev).  Rows of whole 16-byte pieces (kPieces) or whole
+// words (kWords) are read through a buffer over the chunk's rows, so that rows behind the sequence and columns behind the row read
+// as zeros without a branch; others by element (bf16, B2 H16 N4096, d = dv = 100: 129 us by words, 210 by element; d = dv = 128: 102).
+template <bool F32, int W, int NT, int ROWS>
 struct RowLoader {
   typedef typename DecayOps<F32>::elem elem;
   static constexpr int E = 16 / sizeof(elem), PIECES = W / E, ALL = C * PIECES, NL = (ALL + NT - 1) / NT;
   static constexpr int RPP = NT / PIECES;      // rows between a thread's pieces, which have one column
   static_assert(NT % PIECES == 0, "a column per thread");
   u32x4 x[NL];
-  int off;              // of the first piece, in bytes
-  int rb;               // bytes between tokens (VEC)
+  static constexpr int LOADS = ROWS == kPieces ? 1 : 4;      // of a piece
+  int off[LOADS];       // of the first piece, in bytes
+  int rb;               // bytes between tokens (kPieces, kWords)
   const elem* p;        // the next chunk's first row in memory, as if it had 64
   long long row;        // elements between tokens
   int w, move;          // move: tokens in memory from one chunk to the next
@@ -133,17 +138,26 @@ struct RowLoader {
     rb = (int)(row * sizeof(elem));
     p = static_cast<const elem*>(t.p) + b * t.s[0] + h * t.s[1] + (rev ? len - first - C : first) * row;
     const int r = tid / PIECES, col = tid % PIECES * E;
-    off = r < C && col < w ? (rev ? C - 1 - r : r) * rb + col * (int)sizeof(elem) : kOffOutOfRange;
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j)
+      off[j] = r < C && col + j * (E / 4) < w ? (rev ? C - 1 - r : r) * rb + col * (int)sizeof(elem) + 4 * j : kOffOutOfRange;
   }
   // the next chunk, of n >= 1 rows; the others zeros
   __device__ __forceinline__ void load(int n, int rev, int tid) {
-    if (VEC) {
+    if constexpr (ROWS != kElements) {
       // from the end, the n rows are the last of the 64: the buffer starts at them, and earlier ones have negative
       // offsets, which are out of range too, as kOffOutOfRange stays with any of these steps
       const int back = rev ? (C - n) * rb : 0, step = rev ? -RPP * rb : RPP * rb;
       const auto rs = make_rsrc(reinterpret_cast<const char*>(p) + back, (u32)((n - 1) * rb + w * (int)sizeof(elem)));
 #pragma unroll
-      for (int i = 0; i < NL; ++i) x[i] = buf_load_b128(rs, off + (i * step - back));
+      for (int i = 0; i < NL; ++i) {
+        if constexpr (ROWS == kPieces) {
+          x[i] = buf_load_b128(rs, off[0] + (i * step - back));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[i][j] = (u32)__builtin_amdgcn_raw_buffer_load_b32(rs, off[j] + (i * step - back), 0, 0);
+        }
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
@@ -171,8 +185,8 @@ struct RowLoader {
 __device__ __forceinline__ int state_row(int t, int g, int r) { return 32 * (t >> 1) + 8 * g + 4 * (t & 1) + r; }
 
 // One segment.  OUT: outputs (and, with one segment, the last state); else the segment's own state.
-template <bool F32, int DP, int DVP, bool OUT, bool VEC>
-__global__ __launch_bounds__(4 * DVP) __attribute__((amdgpu_waves_per_eu(DP <= 64 && DVP <= 64 && VEC ? 3 : 1))) void decay_kernel(const DecayParams p) {
+template <bool F32, int DP, int DVP, bool OUT, int ROWS>
+__global__ __launch_bounds__(4 * DVP) __attribute__((amdgpu_waves_per_eu(DP <= 64 && DVP <= 64 && ROWS == kPieces ? 3 : 1))) void decay_kernel(const DecayParams p) {
   typedef DecayOps<F32> Ops;
   typedef typename Ops::elem elem;
   typedef typename Ops::frag frag;
@@ -197,8 +211,8 @@ __global__ __launch_bounds__(4 * DVP) __attribute__((amdgpu_waves_per_eu(DP <= 6
   // A segment's own state is a sum in any order: it is taken from the segment's end, so that what this pass read last, the
   // segments' beginnings, is what the outputs' pass reads first, while the memory-side cache still holds it.
   const int begin = OUT || stop <= first ? first : first + (stop - 1 - first) / C * C, step = OUT ? C : -C;
-  RowLoader<F32, DP, NT, VEC> ql, kl;
-  RowLoader<F32, DVP, NT, VEC> vl;
+  RowLoader<F32, DP, NT, ROWS> ql, kl;
+  RowLoader<F32, DVP, NT, ROWS> vl;
   if (OUT) ql.init(job.q, b, h, d, rev, begin, OUT ? 1 : -1, len, tid);
   kl.init(job.k, b, h, d, rev, begin, OUT ? 1 : -1, len, tid);
   vl.init(job.v, b, h, dv, rev, begin, OUT ? 1 : -1, len, tid);
@@ -558,19 +572,25 @@ enum Pass { kStates, kScan, kOutputs };
 template <bool F32, int DP, int DVP>
 void launch_dims(const DecayParams& p, Pass pass, hipStream_t stream) {
   const dim3 grid((unsigned)(p.units * p.njobs)), block(4 * DVP);
-  bool vec = true;
-  for (int j = 0; j < p.njobs; ++j) vec = vec && p.job[j].k.vec && p.job[j].v.vec && (pass != kOutputs || p.job[j].q.vec);
-  if (pass == kScan)
+  if (pass == kScan) {
     hipLaunchKernelGGL((decay_scan_kernel<DP, DVP>), dim3((unsigned)(p.units / p.nseg * (DP * DVP / kScanThreads)), (unsigned)p.njobs),
                        dim3(kScanThreads), 0, stream, p);
-  else if (pass == kStates && vec)
-    hipLaunchKernelGGL((decay_kernel<F32, DP, DVP, false, true>), grid, block, 0, stream, p);
-  else if (pass == kStates)
-    hipLaunchKernelGGL((decay_kernel<F32, DP, DVP, false, false>), grid, block, 0, stream, p);
-  else if (vec)
-    hipLaunchKernelGGL((decay_kernel<F32, DP, DVP, true, true>), grid, block, 0, stream, p);
-  else
-    hipLaunchKernelGGL((decay_kernel<F32, DP, DVP, true, false>), grid, block, 0, stream, p);
+    return;
+  }
+  int rows = kPieces;
+  for (int j = 0; j < p.njobs; ++j) {
+    rows = std::min({rows, p.job[j].k.vec, p.job[j].v.vec});
+    if (pass == kOutputs) rows = std::min(rows, p.job[j].q.vec);
+  }
+#define LA_ROWS(R)                                                                                   \
+  if (rows == R) {                                                                                   \
+    if (pass == kStates)                                                                             \
+      hipLaunchKernelGGL((decay_kernel<F32, DP, DVP, false, R>), grid, block, 0, stream, p);         \
+    else                                                                                             \
+      hipLaunchKernelGGL((decay_kernel<F32, DP, DVP, true, R>), grid, block, 0, stream, p);          \
+  }
+  LA_ROWS(kPieces) LA_ROWS(kWords) LA_ROWS(kElements)
+#undef LA_ROWS
 }
 
 // One pass over the first n of p's jobs, which have the same widths.
@@ -588,10 +608,13 @@ void launch_pass(DecayParams p, int n, Pass pass, hipStream_t stream) {
 
 DecayTensor operand(const void* ptr, const long long* s, int w, bool f32) {
   DecayTensor x{ptr, {s[0], s[1], s[2]}, 0};
-  const int e = f32 ? 4 : 8;
+  auto whole = [&](int bytes) {
+    const int e = bytes / (f32 ? 4 : 2);
+    return reinterpret_cast<uintptr_t>(ptr) % bytes == 0 && w % e == 0 && s[0] % e == 0 && s[1] % e == 0 && s[2] % e == 0;
+  };
   // rows that do not overlap, 64 of them within 2^29 bytes: a buffer's offsets tell rows behind a sequence by their size
-  x.vec = (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && w % e == 0 && s[0] % e == 0 && s[1] % e == 0 && s[2] % e == 0 &&
-          s[2] >= w && s[2] * (f32 ? 4 : 2) <= (1 << 23);
+  const bool buffer = s[2] >= w && s[2] * (f32 ? 4 : 2) <= (1 << 23);
+  x.vec = !buffer ? kElements : whole(16) ? kPieces : whole(4) ? kWords : kElements;
   return x;
 }
 

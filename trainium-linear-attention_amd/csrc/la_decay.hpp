@@ -132,7 +132,7 @@ __device__ __forceinline__ void lds_barrier() {
 struct DecayTensor {
   const void* p;
   long long s[3];
-  int vec;      // rows of 16-byte pieces: start, strides and width allow 16-byte loads
+  int vec;      // how its rows may be read: by element if 0 (start, strides and width allow no more)
 };
 
 }  // namespace la
