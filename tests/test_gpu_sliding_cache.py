@@ -353,3 +353,23 @@ def test_offsets_beyond_32_bits():
     model.check(tail)
     want, A, S = attention(q, tail, (n,), w, 1 / math.sqrt(d))
     close(y, want, A, S, BF, d, w)
+
+
+@pytest.mark.parametrize("dtype,d,dv", [(BF, 100, 60), (BF, 6, 34), (BF, 62, 128), (F32, 63, 5), (F32, 101, 127), (BF, 33, 64)])
+def test_rows_of_words_and_of_elements(dtype, d, dv):
+    """Widths that are no whole 16-byte pieces, in rows that start in the middle of one."""
+    K = _K()
+    g = torch.Generator(device="cuda").manual_seed(d)
+    b, hk, t, start, lengths = 2, 3, 200, (0, 64), (130, 200)
+    rows = [torch.randn(b, hk, t, w + 2, generator=g, device="cuda").to(dtype) for w in (d, dv)]
+    behind = torch.arange(t, device="cuda").view(1, 1, t, 1) >= ints(*lengths).view(b, 1, 1, 1)
+    for shift in (0, 2):
+        k, v = (x[..., shift:x.shape[3] - 2 + shift] for x in rows)
+        if not shift:
+            k, v = k.contiguous(), v.contiguous()
+        cache, model = K.sliding_cache(b, hk, 320, d, dv), Model(b, hk, 5, d, dv)
+        model.append(k, v, list(start), list(lengths))
+        for x in (k, v):      # in place: a view stays one
+            x.masked_fill_(behind, float("nan"))
+        K.sliding_cache_append(cache, k, v, start=ints(*start), lengths=ints(*lengths))
+        model.check(cache)

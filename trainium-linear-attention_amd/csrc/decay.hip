@@ -91,9 +91,6 @@ struct Fade {
   __device__ __forceinline__ float operator()(float x) const { return __builtin_fmaf(x, f, slow ? x : 0.f); }
 };
 
-// How rows are read, by what they and their strides are made of (DecayTensor::vec).
-enum Rows { kElements, kWords, kPieces };
-
 // Where entry (kd, vd) of the head's state lies in state_in.
 __device__ __forceinline__ size_t state_at(int d, int dv, size_t bh, int kd, int vd, int trans) {
   return trans ? (bh * dv + vd) * d + kd : (bh * d + kd) * dv + vd;
@@ -116,7 +113,7 @@ __device__ __forceinline__ int unit_of(const DecayParams& p, int& job) {
 // another: row r of the sequence is token r, or token len - 1 - r (rev).  Rows of whole 16-byte pieces (kPieces) or whole
 // words (kWords) are read through a buffer over the chunk's rows, so that rows behind the sequence and columns behind the row read
 // as zeros without a branch; others by element (bf16, B2 H16 N4096, d = dv = 100: 129 us by words, 210 by element; d = dv = 128: 102).
-template <bool F32, int W, int NT, int ROWS>
+template <bool F32, int W, int NT, Rows ROWS>
 struct RowLoader {
   typedef typename DecayOps<F32>::elem elem;
   static constexpr int E = 16 / sizeof(elem), PIECES = W / E, ALL = C * PIECES, NL = (ALL + NT - 1) / NT;
@@ -185,7 +182,7 @@ struct RowLoader {
 __device__ __forceinline__ int state_row(int t, int g, int r) { return 32 * (t >> 1) + 8 * g + 4 * (t & 1) + r; }
 
 // One segment.  OUT: outputs (and, with one segment, the last state); else the segment's own state.
-template <bool F32, int DP, int DVP, bool OUT, int ROWS>
+template <bool F32, int DP, int DVP, bool OUT, Rows ROWS>
 __global__ __launch_bounds__(4 * DVP) __attribute__((amdgpu_waves_per_eu(DP <= 64 && DVP <= 64 && ROWS == kPieces ? 3 : 1))) void decay_kernel(const DecayParams p) {
   typedef DecayOps<F32> Ops;
   typedef typename Ops::elem elem;
@@ -577,10 +574,10 @@ void launch_dims(const DecayParams& p, Pass pass, hipStream_t stream) {
                        dim3(kScanThreads), 0, stream, p);
     return;
   }
-  int rows = kPieces;
+  Rows rows = kPieces;
   for (int j = 0; j < p.njobs; ++j) {
-    rows = std::min({rows, p.job[j].k.vec, p.job[j].v.vec});
-    if (pass == kOutputs) rows = std::min(rows, p.job[j].q.vec);
+    rows = std::min({rows, p.job[j].k.rows, p.job[j].v.rows});
+    if (pass == kOutputs) rows = std::min(rows, p.job[j].q.rows);
   }
 #define LA_ROWS(R)                                                                                   \
   if (rows == R) {                                                                                   \
@@ -604,18 +601,6 @@ void launch_pass(DecayParams p, int n, Pass pass, hipStream_t stream) {
   LA_DECAY(64, 32) LA_DECAY(64, 64) LA_DECAY(64, 128)
   LA_DECAY(128, 32) LA_DECAY(128, 64) LA_DECAY(128, 128)
 #undef LA_DECAY
-}
-
-DecayTensor operand(const void* ptr, const long long* s, int w, bool f32) {
-  DecayTensor x{ptr, {s[0], s[1], s[2]}, 0};
-  auto whole = [&](int bytes) {
-    const int e = bytes / (f32 ? 4 : 2);
-    return reinterpret_cast<uintptr_t>(ptr) % bytes == 0 && w % e == 0 && s[0] % e == 0 && s[1] % e == 0 && s[2] % e == 0;
-  };
-  // rows that do not overlap, 64 of them within 2^29 bytes: a buffer's offsets tell rows behind a sequence by their size
-  const bool buffer = s[2] >= w && s[2] * (f32 ? 4 : 2) <= (1 << 23);
-  x.vec = !buffer ? kElements : whole(16) ? kPieces : whole(4) ? kWords : kElements;
-  return x;
 }
 
 DecayParams common(const DecayArgs& a) {
@@ -644,9 +629,9 @@ int launch_decay_fwd(const DecayArgs& a, hipStream_t stream) {
   DecayParams p = common(a);
   p.out_f32 = a.out_f32;
   DecayJob& j = p.job[0];
-  j.q = operand(a.q, a.q_strides, a.d, a.in_f32);
-  j.k = operand(a.k, a.k_strides, a.d, a.in_f32);
-  j.v = operand(a.v, a.v_strides, a.dv, a.in_f32);
+  j.q = strided_operand(a.q, a.q_strides, a.d, a.in_f32);
+  j.k = strided_operand(a.k, a.k_strides, a.d, a.in_f32);
+  j.v = strided_operand(a.v, a.v_strides, a.dv, a.in_f32);
   j.out = a.out;
   j.state_in = a.state_in;
   j.state_out = a.state_out;
@@ -669,8 +654,8 @@ int launch_decay_fwd(const DecayArgs& a, hipStream_t stream) {
 // states of the segments, S of (k, v), if the forward pass's are not given, and dS of (q, dy), which the three outputs'
 // pass shares.
 int launch_decay_bwd(const DecayArgs& a, hipStream_t stream) {
-  const DecayTensor q = operand(a.q, a.q_strides, a.d, a.in_f32), k = operand(a.k, a.k_strides, a.d, a.in_f32),
-                    v = operand(a.v, a.v_strides, a.dv, a.in_f32), dy = operand(a.dout, a.dout_strides, a.dv, a.in_f32);
+  const DecayTensor q = strided_operand(a.q, a.q_strides, a.d, a.in_f32), k = strided_operand(a.k, a.k_strides, a.d, a.in_f32),
+                    v = strided_operand(a.v, a.v_strides, a.dv, a.in_f32), dy = strided_operand(a.dout, a.dout_strides, a.dv, a.in_f32);
   DecayParams p = common(a);
   p.out_f32 = a.in_f32;
   auto pass = a.in_f32 ? launch_pass<true> : launch_pass<false>;

@@ -128,11 +128,24 @@ __device__ __forceinline__ void lds_barrier() {
   asm volatile("" ::: "memory");
 }
 
+// How an operand's rows are read, by what start, strides and width are multiples of: 16 bytes, 4 bytes, an element.
+enum Rows { kElements, kWords, kPieces };
+
 // A (B, H, N, w) operand: element (b, h, t, i) at p + b s[0] + h s[1] + t s[2] + i.
 struct DecayTensor {
   const void* p;
   long long s[3];
-  int vec;      // how its rows may be read: by element if 0 (start, strides and width allow no more)
+  Rows rows;
 };
+
+inline DecayTensor strided_operand(const void* p, const long long* s, int w, bool f32) {
+  auto whole = [&](int bytes) {
+    const int e = bytes / (f32 ? 4 : 2);
+    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && w % e == 0 && s[0] % e == 0 && s[1] % e == 0 && s[2] % e == 0;
+  };
+  // rows that do not overlap, 64 of them within 2^29 bytes: a buffer's offsets tell rows behind a sequence by their size
+  const bool buffer = s[2] >= w && s[2] * (f32 ? 4 : 2) <= (1 << 23);
+  return {p, {s[0], s[1], s[2]}, !buffer ? kElements : whole(16) ? kPieces : whole(4) ? kWords : kElements};
+}
 
 }  // namespace la

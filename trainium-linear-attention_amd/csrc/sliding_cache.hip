@@ -72,16 +72,25 @@ struct CacheParams {
 };
 
 // Columns col .. col + E - 1 of row r of a block's new rows from .. to - 1 (x: row `from`), zeros in other rows and behind
-// a row of w.  VEC: through a buffer over these rows, so that no load waits for a branch.
-template <bool F32, bool VEC, int E>
+// a row of w.  Rows of whole pieces or words are read through a buffer over these rows, so that no load waits
+// for a branch (bf16, B8 H16 N4096, d = dv = 100: 71 us by words, 152 by element).
+template <bool F32, Rows ROWS, int E>
 __device__ __forceinline__ void load_row(const void* x, long long stride, int r, int from, int to, int col, int w, float (&y)[E]) {
   constexpr int Z = F32 ? 4 : 2;
-  if constexpr (VEC) {
+  if constexpr (ROWS != kElements) {
     const auto rs = make_rsrc(x, (u32)((to - from - 1) * (int)stride + w) * Z);
     const int at = ((r - from) * (int)stride + col) * Z;
     u32x4 a[E * Z / 16];
 #pragma unroll
-    for (int i = 0; i < E * Z / 16; ++i) a[i] = buf_load_b128(rs, col + i * 16 / Z < w ? at + 16 * i : kOffOutOfRange);
+    for (int i = 0; i < E * Z / 16; ++i) {
+      if constexpr (ROWS == kPieces) {
+        a[i] = buf_load_b128(rs, col + i * 16 / Z < w ? at + 16 * i : kOffOutOfRange);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          a[i][j] = (u32)__builtin_amdgcn_raw_buffer_load_b32(rs, col + (4 * i + j) * 4 / Z < w ? at + 16 * i + 4 * j : kOffOutOfRange, 0, 0);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < E * Z / 16; ++i)
 #pragma unroll
@@ -104,7 +113,7 @@ __device__ __forceinline__ void load_row(const void* x, long long stride, int r,
 // One block of one (sequence, cached head): blockIdx.x the block among those the call touches.  A thread has E columns
 // of a token: 16-byte stores of codes (8 at the narrowest rows, so that every thread has some).  Bound by memory: B8, 8
 // heads of 128, 8200 tokens in bf16 take 74 us (403 MB read and written: 5.4 TB/s), B2, 16 heads of 64, 4096 tokens 11 us.
-template <bool F32, int DP, int DVP, bool VEC>
+template <bool F32, int DP, int DVP, Rows ROWS>
 __global__ __launch_bounds__(256) void cache_append_kernel(const CacheParams p) {
   constexpr int KE = DP >= 64 ? 16 : 8, VE = DVP >= 64 ? 16 : 8, KI = CB * DP / KE / 256, VI = CB * DVP / VE / 256;
   constexpr int KP = DP / KE, VP = DVP / VE, VROW = CB + 4, Z = F32 ? 4 : 2;
@@ -132,12 +141,12 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const CacheParams p) 
 #pragma unroll
   for (int i = 0; i < KI; ++i) {
     const int at = tid + 256 * i;
-    load_row<F32, VEC, KE>(kg, p.k.s[2], at / KP, kept, stop, at % KP * KE, p.d, kx[i]);
+    load_row<F32, ROWS, KE>(kg, p.k.s[2], at / KP, kept, stop, at % KP * KE, p.d, kx[i]);
   }
 #pragma unroll
   for (int i = 0; i < VI; ++i) {
     const int at = tid + 256 * i;
-    load_row<F32, VEC, VE>(vg, p.v.s[2], at / VP, kept, stop, at % VP * VE, p.dv, vx[i]);
+    load_row<F32, ROWS, VE>(vg, p.v.s[2], at / VP, kept, stop, at % VP * VE, p.dv, vx[i]);
   }
 #pragma unroll
   for (int i = 0; i < KI; ++i)
@@ -508,15 +517,12 @@ __global__ __launch_bounds__(DVP < 64 ? 64 : DVP) void cache_combine_kernel(cons
 template <int DP, int DVP>
 int launch_append(const CacheParams& p, int BHK, hipStream_t stream) {
   const dim3 grid((unsigned)((p.N + 2 * CB - 2) / CB), (unsigned)BHK);      // blocks that N tokens may touch
-  const bool vec = p.k.vec && p.v.vec;
-  if (p.in_f32 && vec)
-    hipLaunchKernelGGL((cache_append_kernel<true, DP, DVP, true>), grid, dim3(256), 0, stream, p);
-  else if (p.in_f32)
-    hipLaunchKernelGGL((cache_append_kernel<true, DP, DVP, false>), grid, dim3(256), 0, stream, p);
-  else if (vec)
-    hipLaunchKernelGGL((cache_append_kernel<false, DP, DVP, true>), grid, dim3(256), 0, stream, p);
-  else
-    hipLaunchKernelGGL((cache_append_kernel<false, DP, DVP, false>), grid, dim3(256), 0, stream, p);
+  const Rows rows = std::min(p.k.rows, p.v.rows);
+#define LA_ROWS(F32, R) \
+  if (p.in_f32 == F32 && rows == R) hipLaunchKernelGGL((cache_append_kernel<F32, DP, DVP, R>), grid, dim3(256), 0, stream, p);
+  LA_ROWS(true, kPieces) LA_ROWS(true, kWords) LA_ROWS(true, kElements)
+  LA_ROWS(false, kPieces) LA_ROWS(false, kWords) LA_ROWS(false, kElements)
+#undef LA_ROWS
   return (int)hipGetLastError();
 }
 
@@ -578,14 +584,7 @@ size_t sliding_decode_workspace_bytes(int B, int H, int HK, int dv, int blocks, 
 }
 
 int launch_sliding_append(const SlidingCacheArgs& a, hipStream_t stream) {
-  const int e = a.in_f32 ? 4 : 8;
-  auto operand = [&](const void* ptr, const long long* s, int w) {
-    DecayTensor x{ptr, {s[0], s[1], s[2]}, 0};
-    x.vec = (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && w % e == 0 && s[0] % e == 0 && s[1] % e == 0 && s[2] % e == 0 &&
-            s[2] >= w && s[2] * (32 / e) <= (1 << 23);      // rows apart, 64 of them within a buffer's offsets
-    return x;
-  };
-  const CacheParams p{operand(a.k, a.k_strides, a.d), operand(a.v, a.v_strides, a.dv), static_cast<uint8_t*>(a.kc),
+  const CacheParams p{strided_operand(a.k, a.k_strides, a.d, a.in_f32), strided_operand(a.v, a.v_strides, a.dv, a.in_f32), static_cast<uint8_t*>(a.kc),
                       static_cast<uint8_t*>(a.vc), a.ks, a.vs, a.start, a.lengths, a.last_of ? 1 : 0, a.HK, a.N, a.d, a.dv,
                       a.blocks, a.in_f32 ? 1 : 0};
   return append_dims(p, a.B * a.HK, stream);
