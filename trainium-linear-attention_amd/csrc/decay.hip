@@ -24,7 +24,7 @@
 // chunks on their way instead of one left both passes as they were.  d = dv = 128 is bound by a chunk's chain of
 // LDS reads and matrix products in the one work-group of eight waves that the registers leave a CU: B4 H8 N3001 takes 60 us
 // (16 + 8 + 35); four waves of 32 columns read half as much LDS, but take 370 registers and 15 % longer.  Small calls
-// are two or three launches' latencies: B1 H4 N1024 in fp32 18 us.  The gradients of B2 H16 N8192 at d = dv = 64 take 97 us
+// are two or three launches' latencies: B1 H4 N1024 in fp32 15 us.  The gradients of B2 H16 N8192 at d = dv = 64 take 97 us
 // (17 + 6 + 74) with the states that the forward pass left.
 #include <math.h>
 
@@ -541,11 +541,13 @@ int pad_dim(int x) { return x <= 32 ? 32 : x <= 64 ? 64 : 128; }
 // left over in the last round).
 constexpr int kWgsPerCu = 3;
 // Bytes of a head's segments' states up to which each segment adds up those before it, without a scan: B1 H4 N1024 in fp32 takes
-// 18 us so, 28 with the scan; at B2 H16 N2048, at the limit, the two are equal.
+// 15 us so, 28 with the scan; at B2 H16 N2048, at the limit, the two are equal.
 constexpr int kJoinBytes = 1 << 17;
 
 // Segments of a sequence: enough work-groups for the chip, of at least four chunks, six where a state has more bytes than eight
-// chunks' keys (B4 H8 N3001 at 128 x 128: 61 us, 66 with four and 75 with eight); of two where nothing is scanned.
+// chunks' keys (B4 H8 N3001 at 128 x 128: 61 us, 66 with four and 75 with eight); of two where nothing is scanned, or of one
+// as long as half of the CUs are enough (16 x 64, H4 N300: 9.4 us, 12.5 with two, fp32 11 and 18; H16 N192 at 64 x 64, three chunks:
+// 10.0 and 9.3, fp32 12.5 and 16.5; a group for every CU, B2 H16 N512: 17.7 and 14.6).
 struct Segments {
   int n, chunks;
   bool join;
@@ -555,7 +557,10 @@ Segments segments(long long BH, int N, int d, int dv) {
   const long long want = (long long)kWgsPerCu * device_cu_count() / BH;
   const int least = pad_dim(d) * pad_dim(dv) > 8192 ? 6 : 4;
   long long n = std::min(want, (long long)(chunks / least));
-  if (n < few) n = std::min({want, (long long)(chunks / 2), (long long)few});
+  if (n < few) {
+    const bool single = chunks > 2 && chunks <= few && BH * chunks <= device_cu_count() / 2;
+    n = std::min({want, (long long)(single ? chunks : chunks / 2), (long long)few});
+  }
   n = std::max(1LL, n);
   Segments s{};
   s.chunks = (int)((chunks + n - 1) / n);
