@@ -556,7 +556,7 @@ Segments segments(long long BH, int N, int d, int dv) {
   const int chunks = (N + C - 1) / C, few = kJoinBytes / (pad_dim(d) * pad_dim(dv) * (int)sizeof(float));
   const long long want = (long long)kWgsPerCu * device_cu_count() / BH;
   const int least = pad_dim(d) * pad_dim(dv) > 8192 ? 6 : 4;
-  long long n = std::min(want, (long long)(chunks / least));
+  long long n = std::max(std::min(want, (long long)(chunks / least)), std::min((long long)(chunks / 2), device_cu_count() / BH));
   if (n < few) {
     const bool single = chunks > 2 && chunks <= few && BH * chunks <= device_cu_count() / 2;
     n = std::min({want, (long long)(single ? chunks : chunks / 2), (long long)few});
