@@ -545,9 +545,10 @@ constexpr int kWgsPerCu = 3;
 constexpr int kJoinBytes = 1 << 17;
 
 // Segments of a sequence: enough work-groups for the chip, of at least four chunks, six where a state has more bytes than eight
-// chunks' keys (B4 H8 N3001 at 128 x 128: 61 us, 66 with four and 75 with eight); of two where nothing is scanned, or of one
-// as long as half of the CUs are enough (16 x 64, H4 N300: 9.4 us, 12.5 with two, fp32 11 and 18; H16 N192 at 64 x 64, three chunks:
-// 10.0 and 9.3, fp32 12.5 and 16.5; a group for every CU, B2 H16 N512: 17.7 and 14.6).
+// chunks' keys (B4 H8 N3001 at 128 x 128: 61 us, 66 with four and 75 with eight); but of two as long as there is not one for
+// every CU (bf16 H8 N2048 at 128 x 128: 28 us, 46 with more; fp32 47 and 123), and of one for half of the CUs, if the scan stays
+// short (H8 N1000 at 64 x 64: 13.6 us, 15.7 with two, fp32 16 and 22; three chunks, H16 N192: 10.0 and 9.3, fp32 12.5 and 16.5;
+// one for every CU, B2 H16 N512: 17.7 and 14.6; 128 of one, H2 N8192: 26.5 and 21).
 struct Segments {
   int n, chunks;
   bool join;
@@ -556,11 +557,10 @@ Segments segments(long long BH, int N, int d, int dv) {
   const int chunks = (N + C - 1) / C, few = kJoinBytes / (pad_dim(d) * pad_dim(dv) * (int)sizeof(float));
   const long long want = (long long)kWgsPerCu * device_cu_count() / BH;
   const int least = pad_dim(d) * pad_dim(dv) > 8192 ? 6 : 4;
-  long long n = std::max(std::min(want, (long long)(chunks / least)), std::min((long long)(chunks / 2), device_cu_count() / BH));
-  if (n < few) {
-    const bool single = chunks > 2 && chunks <= few && BH * chunks <= device_cu_count() / 2;
-    n = std::min({want, (long long)(single ? chunks : chunks / 2), (long long)few});
-  }
+  const bool single = chunks > 2 && chunks <= 64 && BH * chunks <= device_cu_count() / 2;
+  const long long most = single ? chunks : chunks / 2;
+  long long n = std::max(std::min(want, (long long)(chunks / least)), std::min(most, device_cu_count() / BH));
+  if (n < few) n = std::min({want, most, (long long)few});
   n = std::max(1LL, n);
   Segments s{};
   s.chunks = (int)((chunks + n - 1) / n);
