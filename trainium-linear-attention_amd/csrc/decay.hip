@@ -22,8 +22,8 @@
 // What bounds it, measured on the device.  d = dv = 64 in bf16 is bound by memory: B1 H16 N65536 takes 185 us, of which the
 // segments' pass 68 (reads 268 MB: 3.9 TB/s), the scan 9, the outputs' pass 106 (536 MB read and written: 5.1 TB/s).  Two
 // chunks on their way instead of one left both passes as they were.  d = dv = 128 is bound by a chunk's chain of
-// LDS reads and matrix products in the one work-group of eight waves that the registers leave a CU: B4 H8 N3001 takes 60 us
-// (16 + 8 + 35); four waves of 32 columns read half as much LDS, but take 370 registers and 15 % longer.  Small calls
+// LDS reads and matrix products in the one work-group of eight waves that the registers leave a CU: B4 H8 N3001 takes 58 us
+// (16 + 8 + 33); four waves of 32 columns read half as much LDS, but take 370 registers and 15 % longer.  Small calls
 // are two or three launches' latencies: B1 H4 N1024 in fp32 15 us.  The gradients of B2 H16 N8192 at d = dv = 64 take 97 us
 // (17 + 6 + 74) with the states that the forward pass left.
 #include <math.h>
