@@ -476,18 +476,23 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(const StepParams p) {
   }
 }
 
-// A head's splits, in order, eight in flight.
+// A head's splits: group j of kJoinGroups takes eight at a time, the 8 j-th and on, all in flight; then the groups in order
+// (one cached head of 128, 131072 tokens, 410 splits: 20.5 us a step, 43 with one group; eight splits are equal).
+constexpr int kJoinGroups = 4;
+constexpr int join_columns(int dvp) { return dvp < 64 ? 64 : dvp; }
 template <int DVP>
-__global__ __launch_bounds__(DVP < 64 ? 64 : DVP) void cache_combine_kernel(const StepParams p) {
+__global__ __launch_bounds__(kJoinGroups * join_columns(DVP)) void cache_combine_kernel(const StepParams p) {
+  constexpr int T = join_columns(DVP);
+  __shared__ float gm[kJoinGroups], gl[kJoinGroups], gy[kJoinGroups][T];
   const size_t head = blockIdx.x;
-  const int c = min((int)threadIdx.x, DVP - 1);
+  const int t = threadIdx.x % T, group = threadIdx.x / T, c = min(t, DVP - 1);
   const float* src = p.part + head * p.splits * (DVP + 2);
   float m = -INFINITY, sum = 0.f, y = 0.f;
-  for (int s0 = 0; s0 < p.splits; s0 += 8) {
+  for (int s0 = 8 * group; s0 < p.splits; s0 += 8 * kJoinGroups) {
     float ms[8], ls[8], os[8], mx = m;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float* part = src + min(s0 + i, p.splits - 1) * (DVP + 2);
+      const float* part = src + (size_t)min(s0 + i, p.splits - 1) * (DVP + 2);
       ms[i] = part[DVP];
       ls[i] = part[DVP + 1];
       os[i] = part[c];
@@ -508,10 +513,27 @@ __global__ __launch_bounds__(DVP < 64 ? 64 : DVP) void cache_combine_kernel(cons
     }
     m = mx;
   }
+  if (t == 0) {
+    gm[group] = m;
+    gl[group] = sum;
+  }
+  gy[group][t] = y;
+  __syncthreads();
   if ((int)threadIdx.x >= p.dv) return;
+  m = gm[0];
+#pragma unroll
+  for (int j = 1; j < kJoinGroups; ++j) m = fmaxf(m, gm[j]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  sum = y = 0.f;
+#pragma unroll
+  for (int j = 0; j < kJoinGroups; ++j) {
+    const float f = exp2_raw(gm[j] - ref);
+    sum = __builtin_fmaf(gl[j], f, sum);
+    y = __builtin_fmaf(gy[j][t], f, y);
+  }
   y = p.lengths[head / p.H] > 0 ? y / sum : 0.f;
-  if (p.out_f32) static_cast<float*>(p.out)[head * p.dv + c] = y;
-  else static_cast<uint16_t*>(p.out)[head * p.dv + c] = f32_to_bf16_bits(y);
+  if (p.out_f32) static_cast<float*>(p.out)[head * p.dv + t] = y;
+  else static_cast<uint16_t*>(p.out)[head * p.dv + t] = f32_to_bf16_bits(y);
 }
 
 template <int DP, int DVP>
@@ -531,7 +553,7 @@ int launch_attn(const StepParams& p, int B, hipStream_t stream) {
   const dim3 grid((unsigned)p.splits, (unsigned)(p.HK * ((p.G + 15) / 16)), (unsigned)B);
   hipLaunchKernelGGL((cache_attn_kernel<F32, DP, DVP>), grid, dim3(256), 0, stream, p);
   if (p.part != nullptr)
-    hipLaunchKernelGGL((cache_combine_kernel<DVP>), dim3((unsigned)(B * p.H)), dim3(DVP < 64 ? 64 : DVP), 0, stream, p);
+    hipLaunchKernelGGL((cache_combine_kernel<DVP>), dim3((unsigned)(B * p.H)), dim3(kJoinGroups * join_columns(DVP)), 0, stream, p);
   return (int)hipGetLastError();
 }
 
